@@ -3,6 +3,9 @@
   vector_add(a, b)             -> a + b          (GPU e2e workload kernel)
   gemm_bf16_nt(a, b, out_fp32) -> a @ b.T        (MFMA 16x16x32 bf16, LDS-tiled)
   gemm_fp8_nt(a, b, out_fp32)  -> a @ b.T        (OCP fp8 e4m3, block-scaled MFMA 16x16x128)
+  mxfp4_quantize(x)            -> q, scale       (OCP microscaled fp4: e2m1 codes, an e8m0 scale for each 32)
+  mxfp4_dequantize(q, scale)   -> x
+  gemm_mxfp4_nt(a, a_scale, b, b_scale, out_fp32) -> a @ b.T  (block-scaled MFMA 16x16x128, native/hip/kamd_mxfp4.hip)
   diag_mfma / diag_hbm / diag_vector_add         (device-plugin burn-in diagnostics)
   Payload(dev)                                    (warm per-GPU payload for GPU pods)
 
@@ -11,6 +14,7 @@ rather than silently falling back to a PyTorch implementation.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -39,6 +43,10 @@ def load():
         L.kamd_vector_add_launch.argtypes = [vp, vp, vp, i, vp]
         L.kamd_gemm_bf16_nt_launch.argtypes = [vp, vp, vp, i, i, i, i, f, i, vp]
         L.kamd_gemm_fp8_nt_launch.argtypes = [vp, vp, vp, i, i, i, i, f, i, vp]
+        i64 = ctypes.c_int64
+        L.kamd_mxfp4_quantize_launch.argtypes = [vp, vp, vp, i64, i64, i64, i, vp]
+        L.kamd_mxfp4_dequantize_launch.argtypes = [vp, vp, vp, i64, i64, i, vp]
+        L.kamd_gemm_mxfp4_nt_launch.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, f, i, vp]
         L.kamd_hbm_copy_launch.argtypes = [vp, vp, sz, vp]
         L.kamd_diag_vector_add.argtypes = [i, i, ctypes.POINTER(ctypes.c_float)]
         L.kamd_diag_mfma.argtypes = [i, i, i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]
@@ -116,6 +124,115 @@ def gemm_fp8_nt(a, b, out_fp32=True, alpha=1.0):
     out = torch.empty((M, N), device=a.device, dtype=torch.float32 if out_fp32 else torch.bfloat16)
     _raise(load().kamd_gemm_fp8_nt_launch(a.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, N, float(alpha),
                                           1 if out_fp32 else 0, _stream(a)), "gemm_fp8_nt")
+    return out
+
+
+MXFP4_BLOCK = 32
+
+
+def _mx_types():
+    import torch
+    return {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _on(t):
+    """Launches go to the tensor's device, whichever is current."""
+    import torch
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _mx_pair(q, scale, what):
+    """Codes and scales as contiguous bytes, `q` 16-byte aligned: views where they are so already."""
+    import torch
+    if q.dtype not in (torch.uint8, torch.float4_e2m1fn_x2):
+        raise ValueError(f"{what}: codes must be uint8 or float4_e2m1fn_x2, got {q.dtype}")
+    if scale.dtype not in (torch.uint8, torch.float8_e8m0fnu):
+        raise ValueError(f"{what}: scales must be uint8 or float8_e8m0fnu, got {scale.dtype}")
+    if q.dim() < 1 or q.dim() != scale.dim() or q.shape[:-1] != scale.shape[:-1] or q.shape[-1] != 16 * scale.shape[-1]:
+        raise ValueError(f"{what}: codes [..., 16 * blocks] need scales [..., blocks], got {tuple(q.shape)} and {tuple(scale.shape)}")
+    if q.device != scale.device:
+        raise ValueError(f"{what}: codes on {q.device}, scales on {scale.device}")
+    q, scale = q.view(torch.uint8).contiguous(), scale.view(torch.uint8).contiguous()
+    return q.clone() if q.data_ptr() % 16 else q, scale
+
+
+def _mx_gpu(t, what):
+    if not t.is_cuda:
+        raise ValueError(f"{what} needs tensors on the GPU, got {t.device}")
+
+
+def mxfp4_quantize(x):
+    """x [..., K] (bf16, fp16 or fp32, any strides) as microscaled fp4: codes [..., 16 * nb] and scales
+    [..., nb], both uint8, nb = ceil(K / 32).
+
+    32 values along the last axis share the scale 2^(s - 127), s = floor(log2(max |x|)) - 2 + 127 and 0 at
+    least; each value is rounded to the nearest of 0 0.5 1 1.5 2 3 4 6 times it (ties to the even code, 6 at
+    most). The lower index is in the low nibble; a last short block is filled with zeros. A block that holds
+    a NaN or an infinity gets s = 255: all of it stands for NaN. No gradient is recorded."""
+    import torch
+    types = _mx_types()
+    if x.dtype not in types:
+        raise ValueError(f"mxfp4_quantize needs bf16, fp16 or fp32, got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError("mxfp4_quantize needs at least one dimension")
+    _mx_gpu(x, "mxfp4_quantize")
+    K = x.shape[-1]
+    nb = -(-K // MXFP4_BLOCK)
+    q = torch.empty((*x.shape[:-1], 16 * nb), device=x.device, dtype=torch.uint8)
+    scale = torch.empty((*x.shape[:-1], nb), device=x.device, dtype=torch.uint8)
+    if x.numel() == 0:
+        return q, scale
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    if x2.stride(1) != 1 and K > 1:
+        x2 = x2.contiguous()
+    with _on(x):
+        _raise(load().kamd_mxfp4_quantize_launch(x2.data_ptr(), q.data_ptr(), scale.data_ptr(), x2.shape[0], K,
+                                                 x2.stride(0), types[x.dtype], _stream(x)), "mxfp4_quantize")
+    return q, scale
+
+
+def mxfp4_dequantize(q, scale, k=None, dtype=None):
+    """The values [..., k] that microscaled fp4 codes [..., 16 * nb] and scales [..., nb] stand for, rounded
+    once to `dtype` (bf16 unless given; fp16, fp32). `k` leaves out what fills the last block; 32 * nb unless
+    given. Scale 255 gives NaN. Codes and scales are uint8 or torch's float4_e2m1fn_x2 and float8_e8m0fnu."""
+    import torch
+    types = _mx_types()
+    dtype = torch.bfloat16 if dtype is None else dtype
+    if dtype not in types:
+        raise ValueError(f"mxfp4_dequantize gives bf16, fp16 or fp32, not {dtype}")
+    q, scale = _mx_pair(q, scale, "mxfp4_dequantize")
+    nb = scale.shape[-1]
+    k = MXFP4_BLOCK * nb if k is None else int(k)
+    if -(-k // MXFP4_BLOCK) != nb or k < 0:
+        raise ValueError(f"mxfp4_dequantize: k={k} does not have {nb} blocks of {MXFP4_BLOCK}")
+    _mx_gpu(q, "mxfp4_dequantize")
+    x = torch.empty((*q.shape[:-1], k), device=q.device, dtype=dtype)
+    if x.numel() == 0:
+        return x
+    with _on(q):
+        _raise(load().kamd_mxfp4_dequantize_launch(q.data_ptr(), scale.data_ptr(), x.data_ptr(), x.numel() // k, k,
+                                                   types[dtype], _stream(q)), "mxfp4_dequantize")
+    return x
+
+
+def gemm_mxfp4_nt(a, a_scale, b, b_scale, out_fp32=True, alpha=1.0):
+    """C = alpha * a @ b.T of microscaled fp4 operands as mxfp4_quantize makes them: a [M, 16 * nb], a_scale
+    [M, nb], b [N, 16 * nb], b_scale [N, nb]; sums in fp32, C fp32 or bf16. Any M and N; K is 32 * nb. A block
+    of scale 255 makes every output that it enters NaN."""
+    import torch
+    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1]:
+        raise ValueError(f"gemm_mxfp4_nt needs codes [M, 16 * blocks] and [N, 16 * blocks], got {tuple(a.shape)} and {tuple(b.shape)}")
+    if a.device != b.device:
+        raise ValueError(f"gemm_mxfp4_nt: a on {a.device}, b on {b.device}")
+    a, a_scale = _mx_pair(a, a_scale, "gemm_mxfp4_nt a")
+    b, b_scale = _mx_pair(b, b_scale, "gemm_mxfp4_nt b")
+    _mx_gpu(a, "gemm_mxfp4_nt")
+    M, N, nb = a.shape[0], b.shape[0], a_scale.shape[1]
+    out = torch.empty((M, N), device=a.device, dtype=torch.float32 if out_fp32 else torch.bfloat16)
+    with _on(a):
+        _raise(load().kamd_gemm_mxfp4_nt_launch(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(),
+                                                out.data_ptr(), M, N, nb, float(alpha), 1 if out_fp32 else 0,
+                                                _stream(a)), "gemm_mxfp4_nt")
     return out
 
 

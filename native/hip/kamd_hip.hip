@@ -15,11 +15,14 @@
 #include <hip/hip_runtime.h>
 #include <type_traits>
 #include <math.h>
+#include <stdarg.h>
 #include <stdint.h>
 #include <stdio.h>
 #include <string.h>
 
 #include <vector>
+
+#include "kamd_hip_err.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -39,6 +42,14 @@ static int check(hipError_t e, const char* what) {
     return -1;
   }
   return 0;
+}
+int kamd_check(hipError_t e, const char* what) { return check(e, what); }
+int kamd_fail(const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof g_err, fmt, ap);
+  va_end(ap);
+  return -1;
 }
 #define HC(x)                              \
   do {                                     \
