@@ -46,7 +46,9 @@ def load():
         i64 = ctypes.c_int64
         L.kamd_mxfp4_quantize_launch.argtypes = [vp, vp, vp, i64, i64, i64, i, vp]
         L.kamd_mxfp4_dequantize_launch.argtypes = [vp, vp, vp, i64, i64, i, vp]
-        L.kamd_gemm_mxfp4_nt_launch.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, f, i, vp]
+        L.kamd_gemm_mxfp4_nt_launch.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, f, i, vp, i64, vp]
+        L.kamd_gemm_mxfp4_nt_workspace.argtypes = [i64, i64, i64]
+        L.kamd_gemm_mxfp4_nt_workspace.restype = i64
         L.kamd_hbm_copy_launch.argtypes = [vp, vp, sz, vp]
         L.kamd_diag_vector_add.argtypes = [i, i, ctypes.POINTER(ctypes.c_float)]
         L.kamd_diag_mfma.argtypes = [i, i, i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]
@@ -229,10 +231,12 @@ def gemm_mxfp4_nt(a, a_scale, b, b_scale, out_fp32=True, alpha=1.0):
     _mx_gpu(a, "gemm_mxfp4_nt")
     M, N, nb = a.shape[0], b.shape[0], a_scale.shape[1]
     out = torch.empty((M, N), device=a.device, dtype=torch.float32 if out_fp32 else torch.bfloat16)
+    need = load().kamd_gemm_mxfp4_nt_workspace(M, N, nb)
+    ws = torch.empty(need, device=a.device, dtype=torch.uint8) if need else None
     with _on(a):
         _raise(load().kamd_gemm_mxfp4_nt_launch(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(),
                                                 out.data_ptr(), M, N, nb, float(alpha), 1 if out_fp32 else 0,
-                                                _stream(a)), "gemm_mxfp4_nt")
+                                                ws.data_ptr() if need else None, need, _stream(a)), "gemm_mxfp4_nt")
     return out
 
 

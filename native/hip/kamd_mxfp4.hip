@@ -245,12 +245,11 @@ __device__ __forceinline__ void tile_of(uint32_t w, int tiles_m, int tiles_n, in
 //   * codes HBM -> LDS without registers (global_load_lds, 16 B a lane), 16-byte slot s of row r holding chunk
 //     s ^ (r / 2 % 8), so that 16 rows' reads of one chunk meet all 64 banks once;
 //   * step s = 0 .. 3 of a tile gives lane l the chunk 4 (l / 32) + s: its four scales are neighbours, one
-//     32-bit word, which the instruction's byte select takes apart;
-//   * scales HBM -> registers -> LDS as [row % 32][half][row / 32], so that a lane has those of all its rows of
-//     a tile in one read. Rows of scales are read at any byte alignment.
+//     32-bit word, which the instruction's byte select takes apart.
 // While a step's products run, the next step's fragments are read into the other register set; the one barrier
 // of a tile stands before its last step, where its last read has returned and the next tile has arrived.
-// B's rows are the instruction's rows, A's its columns: a lane ends with 4 neighbours of a row of C.
+// B's rows are the instruction's rows, A's its columns: a lane ends with 4 neighbours of a row of C. The sums
+// go through LDS once more, so that whole cache lines are stored.
 // Tiles at the lower and right edge are moved up and left into C; what two tiles cover both write alike.
 template <int N, typename F, int... I>
 __device__ __forceinline__ void unroll_(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
@@ -259,9 +258,7 @@ __device__ __forceinline__ void unroll(F f) { unroll_<N>(f, std::make_integer_se
 
 typedef __attribute__((address_space(3))) void lds_void;
 
-template <int T> struct Scales { uint32_t v[T]; };   // of T row groups, 4 blocks each
-
-constexpr int tile_lds(int BM, int BN) { return 2 * (BM + BN) * (128 + 8); }
+constexpr int tile_lds(int BM, int BN) { return 2 * (BM + BN) * 128; }
 
 // acc += a b^T with byte S of the scales. ACC: in place in the accumulation registers. The compiler's own form
 // gives the sum another place and moves it back, which with 256 of them costs more than the products. What
@@ -282,19 +279,54 @@ __device__ __forceinline__ void settle(f32x16& acc) {
   if constexpr (ACC) asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc));
 }
 
-template <typename OutT, int TM, int TN>
+// Scales in the order in which the largest tile's lanes take them: panel (a wave's 128 rows) by tile of K, 64 lanes
+// of 16 bytes, lane (r, h) having 4 blocks of rows r, 32 + r, 64 + r, 96 + r. Read where they lie, a row's 8 bytes a
+// tile cost a cache line each; at 8192^3 that made the product 11 % slower than this kernel and its launch do.
+// Blocks behind the last read as 0, which multiplies zeros.
+__global__ void __launch_bounds__(256)
+arrange_scales_kernel(const uint8_t* __restrict__ As, const uint8_t* __restrict__ Bs, uint8_t* __restrict__ out, int M, int N,
+                      int nb) {
+  const int nt = (nb + 7) / 8, t = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (t >= nt) return;
+  const int r = lane & 31, h = lane >> 5;
+  const int panels_a = (M + 255) / 256 * 2, panel = (int)blockIdx.x;
+  const bool isA = panel < panels_a;
+  const int q = isA ? panel : panel - panels_a, rows = isA ? M : N;
+  const int row0 = min(q / 2 * 256, rows - 256) + q % 2 * 128;
+  const uint8_t* s = (isA ? As : Bs) + (size_t)(row0 + r) * nb;
+  const int c = t * 8 + h * 4;
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint8_t* p = s + (size_t)i * 32 * nb;
+    if (c + 4 <= nb) {
+      __builtin_memcpy(&v[i], p + c, 4);
+    } else {
+      v[i] = 0;
+      for (int k = 0; k < 3; ++k)
+        if (c + k < nb) v[i] |= (uint32_t)p[c + k] << (8 * k);
+    }
+  }
+  __builtin_memcpy(out + (((size_t)panel * nt + t) * 64 + lane) * 16, v, 16);
+}
+
+// ARRANGED: As is what arrange_scales_kernel left, of both operands, and Bs is not used.
+template <typename OutT, int TM, int TN, bool ARRANGED>
 __global__ void __launch_bounds__(256, TM == 4 ? 1 : 2)
 gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, const uint8_t* __restrict__ B,
                  const uint8_t* __restrict__ Bs, OutT* __restrict__ C, int M, int N, int nb, float alpha) {
   constexpr int BM = 64 * TM, BN = 64 * TN;
-  constexpr int DATA = (BM + BN) * 128, SCALE = (BM + BN) * 8;
+  constexpr int DATA = (BM + BN) * 128;
   constexpr bool ACC = TM * TN == 16;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // 2 x codes of A, B; 2 x scales of A, B
+  static_assert(TM == TN, "fragments of A and B are read in pairs");
+  static_assert(!ARRANGED || TM == 4, "scales are arranged for panels of 128 rows");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // 2 x codes of A, B
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, h = lane >> 5;
   const int wm = wave >> 1, wn = wave & 1;
   int tm, tn;
-  tile_of(blockIdx.x, (M + BM - 1) / BM, (N + BN - 1) / BN, tm, tn);
+  const int tiles_m = (M + BM - 1) / BM;
+  tile_of(blockIdx.x, tiles_m, (N + BN - 1) / BN, tm, tn);
   const int m0 = min(tm * BM, M - BM), n0 = min(tn * BN, N - BN);
   const int nt = (nb + 7) / 8, rem = nb - (nt - 1) * 8;   // tiles of K, blocks of the last
 
@@ -312,57 +344,74 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
     __builtin_amdgcn_global_load_lds((const void*)(p + o), (lds_void*)(lds + (t & 1) * DATA + wave * 1024 + j * 4096), 16, 0, 0);
   };
 
-  // scales: a thread takes 8 bytes of a row. Of a short last tile those that end with the row, moved down.
-  constexpr int NS = (BM + BN + 255) / 256;
-  uint64_t sreg[NS];
-  const uint8_t* sp[NS];
-  uint32_t sw[NS];
+  // Scales. Arranged, they are a load of 16 bytes a lane for A and one for B, a tile ahead. Where they lie, a lane
+  // reads a row's 32 bytes of 4 tiles at a time, a batch ahead, and keeps its half of each 8; of a short last tile
+  // it reads the 8 that end with the row, and moves them down.
+  constexpr int GROUPS = TM + TN;
+  struct Scales { uint32_t v[GROUPS]; } sc, sn;   // of A's row groups, then B's: this tile's, the next's
+  uint64_t batch[GROUPS][4];
+  uint32_t queue[GROUPS][4];
+  const uint8_t* sp[GROUPS];
+  if constexpr (ARRANGED) {
+    sp[0] = As + (size_t)(tm * 2 + wm) * nt * 1024 + lane * 16;
+    sp[1] = As + (size_t)((tiles_m + tn) * 2 + wn) * nt * 1024 + lane * 16;
+  } else {
 #pragma unroll
-  for (int n = 0; n < NS; ++n) {
-    const int q = min(wave * 64 + n * 256, BM + BN - 64) + lane;   // a wave without rows repeats the last ones
-    const bool isA = q < BM;
-    const int row = isA ? q : q - BM, T = isA ? TM : TN;
-    sp[n] = (isA ? As + (size_t)(m0 + row) * nb : Bs + (size_t)(n0 + row) * nb);
-    sw[n] = 2 * DATA + (isA ? 0 : BM * 8) + row / (32 * T) * (256 * T) + (row & 31) * (8 * T) + row / 32 % T * 4;
+    for (int n = 0; n < GROUPS; ++n)
+      sp[n] = n < TM ? As + (size_t)(m0 + (wm * TM + n) * 32 + r) * nb : Bs + (size_t)(n0 + (wn * TN + n - TM) * 32 + r) * nb;
   }
-  auto sload = [&](int t, auto last) {
+  auto sload = [&](int t) {
+    if constexpr (ARRANGED) {
+      __builtin_memcpy(&sn.v[0], __builtin_assume_aligned(sp[0] + (size_t)t * 1024, 16), 16);
+      __builtin_memcpy(&sn.v[4], __builtin_assume_aligned(sp[1] + (size_t)t * 1024, 16), 16);
+    } else {
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      __builtin_memcpy(&sreg[n], sp[n] + (size_t)t * 8 - (last ? 8 - rem : 0), 8);
-      if (last) sreg[n] >>= 8 * (8 - rem);
+      for (int n = 0; n < GROUPS; ++n) {
+        const uint8_t* p = sp[n] + (size_t)t * 8;
+        if (t * 8 + 32 <= nb) {
+          __builtin_memcpy(batch[n], p, 32);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (t + i >= nt) continue;
+            const int back = t + i == nt - 1 ? 8 - rem : 0;
+            __builtin_memcpy(&batch[n][i], p + i * 8 - back, 8);
+            batch[n][i] >>= 8 * back;
+          }
+        }
+      }
     }
   };
-  auto swrite = [&](int t) {
+  auto sask = [&](int t) {   // in tile t, for what comes behind it
+    if constexpr (ARRANGED) sload(t + 1);
+    else if (t % 4 == 0 && t + 4 < nt) sload(t + 4);
+  };
+  auto snext = [&](int t) {   // to tile t
+    if constexpr (ARRANGED) {
+      sc = sn;
+    } else {
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      const int T = min(wave * 64 + n * 256, BM + BN - 64) < BM ? TM : TN;
-      *(uint32_t*)(lds + sw[n] + (t & 1) * SCALE) = (uint32_t)sreg[n];
-      *(uint32_t*)(lds + sw[n] + (t & 1) * SCALE + 4 * T) = (uint32_t)(sreg[n] >> 32);
+      for (int n = 0; n < GROUPS; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          queue[n][i] = t % 4 == 0 ? (uint32_t)(h ? batch[n][i] >> 32 : batch[n][i]) : queue[n][i < 3 ? i + 1 : 3];
+        sc.v[n] = queue[n][0];
+      }
     }
   };
 
-  // fragments
-  const int baseA = (wm * 32 * TM + r) * 128, baseB = BM * 128 + (wn * 32 * TN + r) * 128;
-  struct Frags { i32x4 a[TM], b[TN]; } f[2];
-  static_assert(TM == TN, "fragments of A and B are read in pairs");
   // Fragments of step s, two at a time, asked for in the first groups of the step before: the last of them is on its
   // way while the other groups' products run.
+  const int baseA = (wm * 32 * TM + r) * 128, baseB = BM * 128 + (wn * 32 * TN + r) * 128;
+  struct Frags { i32x4 a[TM], b[TN]; } f[2];
   auto read = [&](int t, auto s, int pair) {
-    if (2 * pair >= TM + TN) return;
+    if (2 * pair >= GROUPS) return;
 #pragma unroll
     for (int k = 2 * pair; k < 2 * pair + 2; ++k) {
       const uint8_t* p = lds + (t & 1) * DATA + (((4 * h + s) ^ ((r >> 1) & 7)) << 4);
       if (k % 2 == 0) f[s % 2].b[k / 2] = *(const i32x4*)(p + baseB + k / 2 * 4096);
       else f[s % 2].a[k / 2] = *(const i32x4*)(p + baseA + k / 2 * 4096);
     }
-  };
-  Scales<TM> sa;
-  Scales<TN> sb;
-  auto sread = [&](int t) {
-    const uint8_t* p = lds + 2 * DATA + (t & 1) * SCALE + wm * (256 * TM) + (r * 2 + h) * 4 * TM;
-    __builtin_memcpy(&sa, __builtin_assume_aligned(p, 4 * TM), sizeof sa);
-    p = lds + 2 * DATA + (t & 1) * SCALE + BM * 8 + wn * (256 * TN) + (r * 2 + h) * 4 * TN;
-    __builtin_memcpy(&sb, __builtin_assume_aligned(p, 4 * TN), sizeof sb);
   };
 
   f32x16 acc[TM][TN];
@@ -373,22 +422,23 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  // Step s on one register set, in TM + TN groups: some of the products, then ask(k) asks for something. Asked
-  // for before the first product, it would be in what that product waits for.
-  auto step = [&](auto s, const Scales<TM>& ua, const Scales<TN>& ub, auto ask) {
-    constexpr int GROUPS = TM + TN;
+  // Step s on one register set, in groups: some of the products, then ask(k) asks for something. Asked for before
+  // the first product, it would be in what that product waits for.
+  auto step = [&](auto s, auto ask) {
     unroll<GROUPS>([&](auto k) {
       unroll<TM * TN>([&](auto p) {
         if constexpr (p * GROUPS / (TM * TN) == k)
-          mfma32<ACC, s>(acc[p / TN][p % TN], f[s % 2].b[p % TN], f[s % 2].a[p / TN], ub.v[p % TN], ua.v[p / TN]);
+          mfma32<ACC, s>(acc[p / TN][p % TN], f[s % 2].b[p % TN], f[s % 2].a[p / TN], sc.v[TM + p % TN], sc.v[p / TN]);
       });
       __builtin_amdgcn_sched_barrier(0);
       ask(k);
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  auto landed = [] {   // what this wave asked for is in LDS, what it read is in registers; then everyone's
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  // All but the last KEEP loads that this wave asked for are in LDS, what it read is in registers; then everyone's.
+  auto landed = [](auto keep) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x70 | keep);   // vmcnt(keep) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -399,43 +449,45 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   constexpr std::integral_constant<int, 3> s3{};
   constexpr std::false_type no{};
   constexpr std::true_type yes{};
+  static_assert(LOADS == 2 * GROUPS && LOADS / 2 < 16, "a load for each group of two steps; vmcnt's lower bits");
 
-  // a tile with another behind it; the tile after that is asked for in the last step
-  auto tile = [&](int t, auto fetch, auto last) {
-    step(s0, sa, sb, [&](auto k) { read(t, s1, k); });
-    step(s1, sa, sb, [&](auto k) { read(t, s2, k); });
-    step(s2, sa, sb, [&](auto k) { read(t, s3, k); });
-    swrite(t + 1);
-    landed();
-    const Scales<TM> ua = sa;
-    const Scales<TN> ub = sb;
-    step(s3, ua, ub, [&](auto k) {
-      if constexpr (k == 0) sread(t + 1);
-      read(t + 1, s0, k);
-      if constexpr (fetch) {
-        stage(t + 2, 2 * k, last);
-        stage(t + 2, 2 * k + 1, last);
-        if constexpr (k == TM + TN - 1) sload(t + 2, last);
-      }
+  // A tile with another behind it. The loads of a tile are spread over the last step of the tile two before it and
+  // the first of the tile before it: they pass the vector memory pipe at 16 cycles each for the whole workgroup.
+  auto tile = [&](int t, auto next_last, auto fetch, auto fetch_last) {
+    step(s0, [&](auto k) {
+      read(t, s1, k);
+      stage(t + 1, LOADS / 2 + k, next_last);
+      if constexpr (k == GROUPS - 1) sask(t);
     });
-  };
-  auto fetch = [&](int t, auto last) {
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) stage(t, j, last);
-    sload(t, last);
+    step(s1, [&](auto k) { read(t, s2, k); });
+    step(s2, [&](auto k) { read(t, s3, k); });
+    landed(s0);
+    step(s3, [&](auto k) {
+      read(t + 1, s0, k);
+      if constexpr (fetch) stage(t + 2, k, fetch_last);
+    });
+    snext(t + 1);
   };
 
-  fetch(0, no);
-  swrite(0);
-  landed();
-  if (nt > 2) fetch(1, no);
-  else if (nt == 2) fetch(1, yes);
-  unroll<TM + TN>([&](auto k) { read(0, s0, k); });
-  sread(0);
+  sload(0);
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) stage(0, j, no);
+  if (nt > 1) {
+#pragma unroll
+    for (int j = 0; j < LOADS / 2; ++j) {
+      if (nt > 2) stage(1, j, no);
+      else stage(1, j, yes);
+    }
+    landed(std::integral_constant<int, LOADS / 2>{});
+  } else {
+    landed(s0);
+  }
+  snext(0);
+  unroll<GROUPS>([&](auto k) { read(0, s0, k); });
   int t = 0;
-  for (; t < nt - 3; ++t) tile(t, yes, no);
-  if (t < nt - 2) tile(t++, yes, yes);
-  if (t < nt - 1) tile(t++, no, no);
+  for (; t < nt - 3; ++t) tile(t, no, yes, no);
+  if (t < nt - 2) tile(t++, no, yes, yes);
+  if (t < nt - 1) tile(t++, yes, no, no);
   // the last tile: what is behind the last block is multiplied by zeros
   auto clear = [&](auto s) {
     if (4 * h + s >= rem) {
@@ -444,18 +496,23 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
     }
   };
   clear(s0);
-  step(s0, sa, sb, [&](auto k) { read(t, s1, k); });
+  step(s0, [&](auto k) { read(t, s1, k); });
   clear(s1);
-  step(s1, sa, sb, [&](auto k) { read(t, s2, k); });
+  step(s1, [&](auto k) { read(t, s2, k); });
   clear(s2);
-  step(s2, sa, sb, [&](auto k) { read(t, s3, k); });
+  step(s2, [&](auto k) { read(t, s3, k); });
   clear(s3);
-  step(s3, sa, sb, [&](auto) {});
+  step(s3, [&](auto) {});
+  landed(s0);   // no wave reads codes any more
 
-  // element e of lane (r, h): column r, row 8 (e / 4) + 4 h + e % 4
+  // Element e of lane (r, h) of a 32x32 tile: column r, row 8 (e / 4) + 4 h + e % 4. 32 rows of C go through the
+  // wave's part of LDS at a time, 16 bytes apart from a multiple of the banks.
+  constexpr int ROW = 32 * TN * (int)sizeof(OutT), PITCH = ROW + 16;
+  constexpr int LANES = ROW / 16, ROWS = 64 / LANES;   // of a store
+  static_assert(32 * PITCH <= tile_lds(BM, BN) / 4, "a wave's part of LDS");
+  uint8_t* const mine = lds + wave * (tile_lds(BM, BN) / 4);
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    OutT* p = C + (size_t)(m0 + wm * 32 * TM + i * 32 + r) * N + n0 + wn * 32 * TN + h * 4;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       settle<ACC>(acc[i][j]);
@@ -464,9 +521,18 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
         OutT v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = (OutT)(alpha * acc[i][j][q * 4 + e]);
-        __builtin_memcpy(p + j * 32 + q * 8, v, sizeof v);
+        __builtin_memcpy(__builtin_assume_aligned(mine + r * PITCH + (j * 32 + q * 8 + h * 4) * sizeof(OutT), sizeof v), v, sizeof v);
       }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    uint8_t* p = (uint8_t*)(C + (size_t)(m0 + (wm * TM + i) * 32) * N + n0 + wn * 32 * TN);
+#pragma unroll
+    for (int k = 0; k < 32 / ROWS; ++k) {
+      const int row = k * ROWS + lane / LANES, at = lane % LANES * 16;
+      const i32x4 v = *(const i32x4*)(mine + row * PITCH + at);
+      __builtin_memcpy(p + (size_t)row * N * sizeof(OutT) + at, &v, 16);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
@@ -484,30 +550,66 @@ static int sliced(size_t items, const char* what, F launch) {
   return 0;
 }
 
+// The size of the tiles, in rows and columns: 0 for the small kernel, which takes everything.
+static int tile_size(int64_t M, int64_t N, int64_t nb) {
+  const int64_t least = M < N ? M : N, cus = 256;
+  if (least < 64 || nb < 8 || nb > 1 << 20) return 0;   // whole tiles inside C, 8 blocks to read, 32-bit offsets in a tile
+  auto tiles = [&](int64_t b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
+  if (least >= 256 && tiles(256) >= cus) return 256;
+  if (least >= 128 && tiles(128) >= cus) return 128;
+  return 64;
+}
+
+static int64_t arranged_bytes(int64_t M, int64_t N, int64_t nb) {
+  return ((M + 255) / 256 + (N + 255) / 256) * 2 * ((nb + 7) / 8) * 1024;
+}
+
 template <typename OutT, int T>
-static int launch_tile_of(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
-                          int64_t nb, float alpha, hipStream_t stream) {
+static int launch_tile(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
+                       int64_t nb, float alpha, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   constexpr int BM = 64 * T, LDS = tile_lds(BM, BM);
-  // what the kernel's addresses assume: whole tiles inside C, 8 blocks to read, 32-bit offsets in a tile
-  if (M < BM || N < BM || nb < 8 || nb > 1 << 20) return kamd_fail("gemm_mxfp4_nt: no tile of %d in %lld x %lld x %lld blocks", BM, (long long)M, (long long)N, (long long)nb);
-  // more than 64 KiB of LDS has to be asked for, on every device that the kernel runs on
-  if (LDS > 64 * 1024)
-    HC(hipFuncSetAttribute((const void*)gemm_tile_kernel<OutT, T, T>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+  constexpr bool ARRANGED = T == 4;
+  if (M < BM || N < BM || nb < 8 || nb > 1 << 20)   // what the kernel's addresses assume
+    return kamd_fail("gemm_mxfp4_nt: no tile of %d in %lld x %lld x %lld blocks", BM, (long long)M, (long long)N, (long long)nb);
   const int64_t tiles = ((M + BM - 1) / BM) * ((N + BM - 1) / BM);
   if (tiles >= (int64_t)1 << 24) return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)M, (long long)N);
-  hipLaunchKernelGGL((gemm_tile_kernel<OutT, T, T>), dim3((unsigned)tiles), dim3(256), LDS, stream, (const uint8_t*)A,
-                     (const uint8_t*)As, (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, alpha);
+  auto kernel = gemm_tile_kernel<OutT, T, T, ARRANGED>;
+  if (ARRANGED) {
+    if (!workspace || workspace_bytes < arranged_bytes(M, N, nb) || ((uintptr_t)workspace & 15))
+      return kamd_fail("gemm_mxfp4_nt: needs a workspace of %lld bytes, 16-byte aligned", (long long)arranged_bytes(M, N, nb));
+    // more than 64 KiB of LDS has to be asked for, on every device that the kernel runs on
+    if (LDS > 64 * 1024) HC(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+    const int64_t panels = ((M + 255) / 256 + (N + 255) / 256) * 2;
+    hipLaunchKernelGGL(arrange_scales_kernel, dim3((unsigned)panels, (unsigned)((nb + 31) / 32)), dim3(256), 0, stream,
+                       (const uint8_t*)As, (const uint8_t*)Bs, (uint8_t*)workspace, (int)M, (int)N, (int)nb);
+    HC(hipGetLastError());
+    As = workspace;
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), LDS, stream, (const uint8_t*)A, (const uint8_t*)As,
+                     (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, alpha);
   return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
 }
 
 template <typename OutT>
-static int launch_tile(int T, const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
-                       int64_t nb, float alpha, hipStream_t stream) {
-  switch (T) {
-    case 1: return launch_tile_of<OutT, 1>(A, As, B, Bs, C, M, N, nb, alpha, stream);
-    case 2: return launch_tile_of<OutT, 2>(A, As, B, Bs, C, M, N, nb, alpha, stream);
-    default: return launch_tile_of<OutT, 4>(A, As, B, Bs, C, M, N, nb, alpha, stream);
+static int launch_gemm(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N, int64_t nb,
+                       float alpha, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  if (nb == 0) {
+    const size_t n = (size_t)M * N;
+    if (n > SLICE) return kamd_fail("gemm_mxfp4_nt: an empty K with more than 2^31 outputs");
+    hipLaunchKernelGGL(zero_kernel<OutT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, (OutT*)C, n);
+    return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
   }
+  switch (tile_size(M, N, nb)) {
+    case 256: return launch_tile<OutT, 4>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);
+    case 128: return launch_tile<OutT, 2>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream);
+    case 64: return launch_tile<OutT, 1>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream);
+  }
+  const int64_t tiles = ((M + 15) / 16) * ((N + 15) / 16);
+  if (tiles * (SMALL_WAVES * 64) >= (int64_t)1 << 32)
+    return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)M, (long long)N);
+  hipLaunchKernelGGL(gemm_small_kernel<OutT>, dim3((unsigned)tiles), dim3(SMALL_WAVES * 64), 0, stream, (const uint8_t*)A,
+                     (const uint8_t*)As, (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, alpha);
+  return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
 }
 }  // namespace mxfp4
 
@@ -548,43 +650,23 @@ int kamd_mxfp4_dequantize_launch(const void* q, const void* scale, void* x, int6
   });
 }
 
+// bytes of scratch memory that the product of these sizes needs, 0 for most
+int64_t kamd_gemm_mxfp4_nt_workspace(int64_t M, int64_t N, int64_t nb) {
+  return M > 0 && N > 0 && nb > 0 && mxfp4::tile_size(M, N, nb) == 256 ? mxfp4::arranged_bytes(M, N, nb) : 0;
+}
+
 // C[M, N] = alpha * A B^T, A [M, 16 nb] / As [M, nb], B [N, 16 nb] / Bs [N, nb] contiguous, A and B 16-byte aligned;
-// C fp32 or bf16, contiguous. nb = 0 gives zeros.
+// C fp32 or bf16, contiguous. nb = 0 gives zeros. The workspace is 16-byte aligned and used in stream order.
 int kamd_gemm_mxfp4_nt_launch(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
-                              int64_t nb, float alpha, int out_fp32, hipStream_t stream) {
-  using namespace mxfp4;
+                              int64_t nb, float alpha, int out_fp32, void* workspace, int64_t workspace_bytes,
+                              hipStream_t stream) {
   const int64_t most = (int64_t)1 << 27;
   if (M < 0 || N < 0 || nb < 0 || M > most || N > most || nb > most)
     return kamd_fail("gemm_mxfp4_nt: sizes out of range (%lld x %lld x %lld blocks)", (long long)M, (long long)N, (long long)nb);
   if (M == 0 || N == 0) return 0;
   if ((((uintptr_t)A) | ((uintptr_t)B)) & 15) return kamd_fail("gemm_mxfp4_nt: A/B must be 16-byte aligned");
-  if (nb == 0) {
-    const size_t n = (size_t)M * N;
-    if (n > SLICE) return kamd_fail("gemm_mxfp4_nt: an empty K with more than 2^31 outputs");
-    if (out_fp32)
-      hipLaunchKernelGGL(zero_kernel<float>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, (float*)C, n);
-    else
-      hipLaunchKernelGGL(zero_kernel<__bf16>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, (__bf16*)C, n);
-    return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
-  }
-  if (nb >= 8 && nb <= 1 << 20 && M >= 64 && N >= 64) {
-    // ROUTE
-    const int cus = 256;
-    int T = 1;
-    if (M >= 128 && N >= 128 && ((M + 127) / 128) * ((N + 127) / 128) >= cus) T = 2;
-    if (M >= 256 && N >= 256 && ((M + 255) / 256) * ((N + 255) / 256) >= cus) T = 4;
-    return out_fp32 ? launch_tile<float>(T, A, As, B, Bs, C, M, N, nb, alpha, stream)
-                    : launch_tile<__bf16>(T, A, As, B, Bs, C, M, N, nb, alpha, stream);
-  }
-  const int64_t tiles = ((M + 15) / 16) * ((N + 15) / 16);
-  if (tiles * (SMALL_WAVES * 64) >= (int64_t)1 << 32) return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)M, (long long)N);
-  if (out_fp32)
-    hipLaunchKernelGGL(gemm_small_kernel<float>, dim3((unsigned)tiles), dim3(SMALL_WAVES * 64), 0, stream, (const uint8_t*)A,
-                       (const uint8_t*)As, (const uint8_t*)B, (const uint8_t*)Bs, (float*)C, (int)M, (int)N, (int)nb, alpha);
-  else
-    hipLaunchKernelGGL(gemm_small_kernel<__bf16>, dim3((unsigned)tiles), dim3(SMALL_WAVES * 64), 0, stream, (const uint8_t*)A,
-                       (const uint8_t*)As, (const uint8_t*)B, (const uint8_t*)Bs, (__bf16*)C, (int)M, (int)N, (int)nb, alpha);
-  return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
+  return out_fp32 ? mxfp4::launch_gemm<float>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream)
+                  : mxfp4::launch_gemm<__bf16>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -277,7 +277,8 @@ def test_gemm(gpu, M, N, nb):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("M,N,K", [(4096, 4096, 4096), (2048, 1024, 4096), (8192, 512, 1024), (1, 8192, 7264), (32, 4096, 4096),
-                                   (300, 4096, 2048), (1000, 520, 264), (3000, 3001, 1111)])
+                                   (300, 4096, 2048), (1000, 520, 264), (3000, 3001, 1111), (4097, 4095, 289),
+                                   (4352, 4100, 1000), (8191, 2100, 600), (2100, 8200, 512), (4096, 4096, 256), (4096, 4096, 768)])
 def test_gemm_large(gpu, M, N, K):
     """Exact as above; the oracle is a product in 64 bits on the GPU, whose sums of these are exact too."""
     a, sa = operand(M, -(-K // 32), 3)
@@ -358,7 +359,8 @@ def test_gemm_operands_as_they_come(gpu, M):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,N,nb", [(3, 50, 9), (70, 33, 17), (300, 400, 13), (513, 300, 20)])
+@pytest.mark.parametrize("M,N,nb", [(3, 50, 9), (70, 33, 17), (300, 400, 13), (513, 300, 20), (2100, 2050, 9),
+                                    (4100, 4111, 13)])
 def test_gemm_writes_its_output_and_nothing_else(gpu, M, N, nb):
     """Launched into the middle of a larger buffer, the bytes before and behind stay."""
     a, sa = operand(M, nb, 12)
@@ -366,9 +368,12 @@ def test_gemm_writes_its_output_and_nothing_else(gpu, M, N, nb):
     for fp32, dtype in ((1, torch.float32), (0, torch.bfloat16)):
         buf = torch.full((M * N + 512,), 3.0, device=gpu, dtype=dtype)
         out = buf[256:256 + M * N]
+        need = hk.load().kamd_gemm_mxfp4_nt_workspace(M, N, nb)
+        ws = torch.full((need + 512,), 77, device=gpu, dtype=torch.uint8)
         rc = hk.load().kamd_gemm_mxfp4_nt_launch(a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(), out.data_ptr(),
-                                                 M, N, nb, 1.0, fp32, hk._stream(a))
+                                                 M, N, nb, 1.0, fp32, ws.data_ptr() + 256, need, hk._stream(a))
         assert rc == 0
+        assert (ws[:256] == 77).all() and (ws[256 + need:] == 77).all()
         assert (buf[:256] == 3).all() and (buf[256 + M * N:] == 3).all()
         assert torch.equal(out.view(M, N).cpu(), product(a, sa, b, sb).float().to(dtype))
 
@@ -502,8 +507,13 @@ def test_c_entries_refuse_bad_sizes():
     assert L.kamd_mxfp4_quantize_launch(0, 0, 0, 1, 1 << 40, 32, 0, None) == -1
     assert b"too large" in L.kamd_hip_last_error()
     assert L.kamd_mxfp4_dequantize_launch(0, 0, 0, 1, -1, 0, None) == -1
-    assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, -1, 1, 1, 1.0, 1, None) == -1
-    assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, 1, 1 << 40, 1, 1.0, 1, None) == -1
-    assert L.kamd_gemm_mxfp4_nt_launch(8, 0, 16, 0, 0, 1, 1, 1, 1.0, 1, None) == -1
+    assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, -1, 1, 1, 1.0, 1, None, 0, None) == -1
+    assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, 1, 1 << 40, 1, 1.0, 1, None, 0, None) == -1
+    assert L.kamd_gemm_mxfp4_nt_launch(8, 0, 16, 0, 0, 1, 1, 1, 1.0, 1, None, 0, None) == -1
     assert b"aligned" in L.kamd_hip_last_error()
-    assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, 0, 1, 1, 1.0, 1, None) == 0
+    assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, 0, 1, 1, 1.0, 1, None, 0, None) == 0
+    need = L.kamd_gemm_mxfp4_nt_workspace(8192, 8192, 256)
+    assert need >= 2 * 8192 * 256 and L.kamd_gemm_mxfp4_nt_workspace(1, 8192, 256) == 0
+    for ws, size in ((None, need), (16, need - 1), (8, need)):
+        assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, 8192, 8192, 256, 1.0, 1, ws, size, None) == -1
+        assert b"workspace" in L.kamd_hip_last_error()
