@@ -241,7 +241,7 @@ __device__ __forceinline__ void tile_of(uint32_t w, int tiles_m, int tiles_n, in
 // ---------------------------------------------------------------------------
 // Large products. A workgroup of 4 waves makes a BM x BN tile of C, each wave a quarter of TM x TN tiles of
 // 32x32 (v_mfma_scale_f32_32x32x64_f8f6f4: lane l holds chunk l / 32 of row l % 32 and that block's scale).
-// K goes by in tiles of 8 blocks (256 values, 128 B a row), two of them in LDS:
+// K goes by in tiles of 8 blocks (256 values, 128 B a row), STAGES of them in LDS:
 //   * codes HBM -> LDS without registers (global_load_lds, 16 B a lane), 16-byte slot s of row r holding chunk
 //     s ^ (r / 2 % 8), so that 16 rows' reads of one chunk meet all 64 banks once;
 //   * step s = 0 .. 3 of a tile gives lane l the chunk 4 (l / 32) + s: its four scales are neighbours, one
@@ -258,7 +258,7 @@ __device__ __forceinline__ void unroll(F f) { unroll_<N>(f, std::make_integer_se
 
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr int tile_lds(int BM, int BN) { return 2 * (BM + BN) * 128; }
+constexpr int tile_lds(int BM, int BN, int stages) { return stages * (BM + BN) * 128; }
 
 // acc += a b^T with byte S of the scales. ACC: in place in the accumulation registers. The compiler's own form
 // gives the sum another place and moves it back, which with 256 of them costs more than the products. What
@@ -282,36 +282,51 @@ __device__ __forceinline__ void settle(f32x16& acc) {
 // Scales in the order in which the largest tile's lanes take them: panel (a wave's 128 rows) by tile of K, 64 lanes
 // of 16 bytes, lane (r, h) having 4 blocks of rows r, 32 + r, 64 + r, 96 + r. Read where they lie, a row's 8 bytes a
 // tile cost a cache line each; at 8192^3 that made the product 11 % slower than this kernel and its launch do.
-// Blocks behind the last read as 0, which multiplies zeros.
+// A workgroup turns 8 tiles of a panel, 64 bytes a row, over in LDS. Blocks behind the last read as 0, which
+// multiplies zeros.
 __global__ void __launch_bounds__(256)
 arrange_scales_kernel(const uint8_t* __restrict__ As, const uint8_t* __restrict__ Bs, uint8_t* __restrict__ out, int M, int N,
                       int nb) {
-  const int nt = (nb + 7) / 8, t = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (t >= nt) return;
-  const int r = lane & 31, h = lane >> 5;
+  constexpr int PITCH = 68;   // 17 banks: 32 rows' words of one tile lie in different ones
+  __shared__ uint8_t rows[128 * PITCH];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+  const int nt = (nb + 7) / 8, t0 = (int)blockIdx.y * 8;
   const int panels_a = (M + 255) / 256 * 2, panel = (int)blockIdx.x;
   const bool isA = panel < panels_a;
-  const int q = isA ? panel : panel - panels_a, rows = isA ? M : N;
-  const int row0 = min(q / 2 * 256, rows - 256) + q % 2 * 128;
-  const uint8_t* s = (isA ? As : Bs) + (size_t)(row0 + r) * nb;
-  const int c = t * 8 + h * 4;
-  uint32_t v[4];
+  const int q = isA ? panel : panel - panels_a, all = isA ? M : N;
+  const int row0 = min(q / 2 * 256, all - 256) + q % 2 * 128;
+  const uint8_t* s = isA ? As : Bs;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint8_t* p = s + (size_t)i * 32 * nb;
-    if (c + 4 <= nb) {
-      __builtin_memcpy(&v[i], p + c, 4);
+  for (int i = 0; i < 2; ++i) {
+    const int row = i * 64 + tid / 4, c = t0 * 8 + tid % 4 * 16;
+    const uint8_t* p = s + (size_t)(row0 + row) * nb + c;
+    uint32_t v[4] = {0, 0, 0, 0};
+    if (c + 16 <= nb) {
+      __builtin_memcpy(v, p, 16);
     } else {
-      v[i] = 0;
-      for (int k = 0; k < 3; ++k)
-        if (c + k < nb) v[i] |= (uint32_t)p[c + k] << (8 * k);
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (c + k < nb) v[k / 4] |= (uint32_t)p[k] << (8 * (k % 4));
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *(uint32_t*)(rows + row * PITCH + tid % 4 * 16 + k * 4) = v[k];
   }
-  __builtin_memcpy(out + (((size_t)panel * nt + t) * 64 + lane) * 16, v, 16);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t = i * 4 + tid / 64;
+    if (t0 + t >= nt) continue;
+    uint32_t v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = *(const uint32_t*)(rows + (k * 32 + r) * PITCH + t * 8 + h * 4);
+    __builtin_memcpy(__builtin_assume_aligned(out + (((size_t)panel * nt + t0 + t) * 64 + lane) * 16, 16), v, 16);
+  }
 }
 
 // ARRANGED: As is what arrange_scales_kernel left, of both operands, and Bs is not used.
-template <typename OutT, int TM, int TN, bool ARRANGED>
+constexpr int waitcnt(int vm, int lgkm) { return (vm & 15) | (vm >> 4) << 14 | 7 << 4 | lgkm << 8; }   // s_waitcnt's operand
+
+template <typename OutT, int TM, int TN, int STAGES, bool ARRANGED>
 __global__ void __launch_bounds__(256, TM == 4 ? 1 : 2)
 gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, const uint8_t* __restrict__ B,
                  const uint8_t* __restrict__ Bs, OutT* __restrict__ C, int M, int N, int nb, float alpha) {
@@ -320,7 +335,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   constexpr bool ACC = TM * TN == 16;
   static_assert(TM == TN, "fragments of A and B are read in pairs");
   static_assert(!ARRANGED || TM == 4, "scales are arranged for panels of 128 rows");
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // 2 x codes of A, B
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // STAGES x codes of A, B
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, h = lane >> 5;
   const int wm = wave >> 1, wn = wave & 1;
@@ -337,20 +352,21 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   const uint8_t* const tA = A + (size_t)m0 * row_bytes;
   const uint8_t* const tB = B + (size_t)n0 * row_bytes;
   constexpr int LOADS = (BM + BN) / 32;
-  auto stage = [&](int t, int j, auto last) {
+  auto stage = [&](int t, int buffer, int j, bool inner = false) {
     uint32_t o = off;
-    if (last && chunk >= rem) o -= (uint32_t)(chunk - rem + 1) * 16;   // behind the last block: that one again
+    if (!inner && t == nt - 1 && chunk >= rem) o -= (uint32_t)(chunk - rem + 1) * 16;   // behind the last block: that one again
     const uint8_t* p = (j < BM / 32 ? tA + j * 32 * row_bytes : tB + (j - BM / 32) * 32 * row_bytes) + (size_t)t * 128;
-    __builtin_amdgcn_global_load_lds((const void*)(p + o), (lds_void*)(lds + (t & 1) * DATA + wave * 1024 + j * 4096), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((const void*)(p + o), (lds_void*)(lds + buffer * DATA + wave * 1024 + j * 4096), 16, 0, 0);
   };
 
-  // Scales. Arranged, they are a load of 16 bytes a lane for A and one for B, a tile ahead. Where they lie, a lane
-  // reads a row's 32 bytes of 4 tiles at a time, a batch ahead, and keeps its half of each 8; of a short last tile
-  // it reads the 8 that end with the row, and moves them down.
+  // Scales. Arranged, they are a load of 16 bytes a lane for A and one for B, a tile ahead. Where they lie, a row's
+  // 32 bytes of 4 tiles are read at a time, a batch ahead, lane (r, h) taking tiles 2 h and 2 h + 1; the halves of the
+  // wave then swap, each keeping its half of every 8 bytes. Of a short last tile the 8 bytes that end with the row
+  // are read, and moved down.
   constexpr int GROUPS = TM + TN;
   struct Scales { uint32_t v[GROUPS]; } sc, sn;   // of A's row groups, then B's: this tile's, the next's
-  uint64_t batch[GROUPS][4];
-  uint32_t queue[GROUPS][4];
+  uint64_t batch[GROUPS][2];
+  Scales queue[4];
   const uint8_t* sp[GROUPS];
   if constexpr (ARRANGED) {
     sp[0] = As + (size_t)(tm * 2 + wm) * nt * 1024 + lane * 16;
@@ -367,14 +383,15 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
     } else {
 #pragma unroll
       for (int n = 0; n < GROUPS; ++n) {
-        const uint8_t* p = sp[n] + (size_t)t * 8;
+        const uint8_t* p = sp[n] + (size_t)t * 8 + h * 16;
         if (t * 8 + 32 <= nb) {
-          __builtin_memcpy(batch[n], p, 32);
+          __builtin_memcpy(batch[n], p, 16);
         } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (t + i >= nt) continue;
-            const int back = t + i == nt - 1 ? 8 - rem : 0;
+          for (int i = 0; i < 2; ++i) {
+            const int at = t + h * 2 + i;
+            if (at >= nt) continue;
+            const int back = at == nt - 1 ? 8 - rem : 0;
             __builtin_memcpy(&batch[n][i], p + i * 8 - back, 8);
             batch[n][i] >>= 8 * back;
           }
@@ -382,21 +399,28 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
       }
     }
   };
-  auto sask = [&](int t) {   // in tile t, for what comes behind it
-    if constexpr (ARRANGED) sload(t + 1);
-    else if (t % 4 == 0 && t + 4 < nt) sload(t + 4);
+  auto sask = [&](int t, auto u) {   // in tile t, u = t % 4, for what comes behind it
+    if constexpr (ARRANGED) {
+      if (t + 1 < nt) sload(t + 1);
+    } else if constexpr (u == 0) {
+      if (t + 4 < nt) sload(t + 4);
+    }
   };
-  auto snext = [&](int t) {   // to tile t
+  auto snext = [&](auto u) {   // to a tile t with u = t % 4
     if constexpr (ARRANGED) {
       sc = sn;
     } else {
+      if constexpr (u == 0) {
 #pragma unroll
-      for (int n = 0; n < GROUPS; ++n) {
+        for (int n = 0; n < GROUPS; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          queue[n][i] = t % 4 == 0 ? (uint32_t)(h ? batch[n][i] >> 32 : batch[n][i]) : queue[n][i < 3 ? i + 1 : 3];
-        sc.v[n] = queue[n][0];
+          for (int i = 0; i < 2; ++i) {
+            const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap((uint32_t)batch[n][i], (uint32_t)(batch[n][i] >> 32), false, false));
+            queue[i].v[n] = v.x;
+            queue[2 + i].v[n] = v.y;
+          }
       }
+      sc = queue[u];
     }
   };
 
@@ -404,11 +428,11 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   // way while the other groups' products run.
   const int baseA = (wm * 32 * TM + r) * 128, baseB = BM * 128 + (wn * 32 * TN + r) * 128;
   struct Frags { i32x4 a[TM], b[TN]; } f[2];
-  auto read = [&](int t, auto s, int pair) {
+  auto read = [&](int buffer, auto s, int pair) {
     if (2 * pair >= GROUPS) return;
 #pragma unroll
     for (int k = 2 * pair; k < 2 * pair + 2; ++k) {
-      const uint8_t* p = lds + (t & 1) * DATA + (((4 * h + s) ^ ((r >> 1) & 7)) << 4);
+      const uint8_t* p = lds + buffer * DATA + (((4 * h + s) ^ ((r >> 1) & 7)) << 4);
       if (k % 2 == 0) f[s % 2].b[k / 2] = *(const i32x4*)(p + baseB + k / 2 * 4096);
       else f[s % 2].a[k / 2] = *(const i32x4*)(p + baseA + k / 2 * 4096);
     }
@@ -438,7 +462,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   // All but the last KEEP loads that this wave asked for are in LDS, what it read is in registers; then everyone's.
   auto landed = [](auto keep) {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x70 | keep);   // vmcnt(keep) lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(waitcnt(keep, 0));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -449,68 +473,87 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   constexpr std::integral_constant<int, 3> s3{};
   constexpr std::false_type no{};
   constexpr std::true_type yes{};
-  static_assert(LOADS == 2 * GROUPS && LOADS / 2 < 16, "a load for each group of two steps; vmcnt's lower bits");
+  static_assert(LOADS == 2 * GROUPS, "a load for each group of two steps");
 
-  // A tile with another behind it. The loads of a tile are spread over the last step of the tile two before it and
-  // the first of the tile before it: they pass the vector memory pipe at 16 cycles each for the whole workgroup.
-  auto tile = [&](int t, auto next_last, auto fetch, auto fetch_last) {
+  // Tile t in buffer u % STAGES, u = t % 4. The loads of a tile are spread over the last step of the tile STAGES
+  // before it and the first of the next one: they pass the vector memory pipe at 16 cycles each for the whole
+  // workgroup. full: all tiles that it asks for are there; else it sees which are, and whether it is the last.
+  // INNER: full ones do not ask for the last either, whose loads take some more instructions (256 tile: 1.5 %).
+  constexpr bool INNER = ARRANGED;
+  auto tile = [&](int t, auto u, auto full) {
+    constexpr int HERE = u % STAGES, NEXT = (u + 1) % STAGES, BEFORE = (u + STAGES - 1) % STAGES;
+    const bool next = full || t + 1 < nt;
+    auto clear = [&](auto s) {   // what is behind the last block is multiplied by zeros
+      if (!full && !next && 4 * h + s >= rem) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) f[s % 2].a[i] = i32x4{0, 0, 0, 0};
+      }
+    };
+    clear(s0);
     step(s0, [&](auto k) {
-      read(t, s1, k);
-      stage(t + 1, LOADS / 2 + k, next_last);
-      if constexpr (k == GROUPS - 1) sask(t);
+      read(HERE, s1, k);
+      if (full || t + STAGES - 1 < nt) stage(t + STAGES - 1, BEFORE, LOADS / 2 + k, full && INNER);
+      if constexpr (k == 0) sask(t, u);
     });
-    step(s1, [&](auto k) { read(t, s2, k); });
-    step(s2, [&](auto k) { read(t, s3, k); });
-    landed(s0);
+    clear(s1);
+    step(s1, [&](auto k) { read(HERE, s2, k); });
+    clear(s2);
+    step(s2, [&](auto k) { read(HERE, s3, k); });
+    if (full) {
+      landed(std::integral_constant<int, (STAGES - 2) * LOADS>{});
+    } else if (STAGES > 2 && t + 3 < nt) {
+      landed(std::integral_constant<int, STAGES == 4 ? 2 * LOADS : 0>{});
+    } else if (STAGES > 2 && t + 2 < nt) {
+      landed(std::integral_constant<int, STAGES == 4 ? LOADS : 0>{});
+    } else {
+      landed(s0);
+    }
+    clear(s3);
     step(s3, [&](auto k) {
-      read(t + 1, s0, k);
-      if constexpr (fetch) stage(t + 2, k, fetch_last);
+      if (next) read(NEXT, s0, k);
+      if (full || t + STAGES < nt) stage(t + STAGES, HERE, k, full && INNER);
     });
-    snext(t + 1);
+    if (next) snext(std::integral_constant<int, (u + 1) % 4>{});
+    return next;
   };
+  static_assert(STAGES == 2 || STAGES == 4, "a buffer follows from t % 4");
 
   sload(0);
 #pragma unroll
-  for (int j = 0; j < LOADS; ++j) stage(0, j, no);
-  if (nt > 1) {
+  for (int j = 0; j < LOADS; ++j) stage(0, 0, j);
+  // The scales have come. Said outside of any branch: on a path that it took for possible the compiler saw them on
+  // their way into the loop, and waited there for all loads, every time.
+  __builtin_amdgcn_s_waitcnt(waitcnt(LOADS, 15));
+  snext(s0);
 #pragma unroll
-    for (int j = 0; j < LOADS / 2; ++j) {
-      if (nt > 2) stage(1, j, no);
-      else stage(1, j, yes);
-    }
-    landed(std::integral_constant<int, LOADS / 2>{});
-  } else {
-    landed(s0);
-  }
-  snext(0);
+  for (int i = 1; i < STAGES; ++i)
+#pragma unroll
+    for (int j = 0; j < (i < STAGES - 1 ? LOADS : LOADS / 2); ++j)
+      if (i < nt) stage(i, i, j);
+  if (nt >= STAGES) landed(std::integral_constant<int, (STAGES - 2) * LOADS + LOADS / 2>{});
+  else landed(s0);
   unroll<GROUPS>([&](auto k) { read(0, s0, k); });
   int t = 0;
-  for (; t < nt - 3; ++t) tile(t, no, yes, no);
-  if (t < nt - 2) tile(t++, no, yes, yes);
-  if (t < nt - 1) tile(t++, yes, no, no);
-  // the last tile: what is behind the last block is multiplied by zeros
-  auto clear = [&](auto s) {
-    if (4 * h + s >= rem) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i) f[s % 2].a[i] = i32x4{0, 0, 0, 0};
-    }
-  };
-  clear(s0);
-  step(s0, [&](auto k) { read(t, s1, k); });
-  clear(s1);
-  step(s1, [&](auto k) { read(t, s2, k); });
-  clear(s2);
-  step(s2, [&](auto k) { read(t, s3, k); });
-  clear(s3);
-  step(s3, [&](auto) {});
+  for (; t + 3 + STAGES + INNER < nt; t += 4) {
+    tile(t, s0, yes);
+    tile(t + 1, s1, yes);
+    tile(t + 2, s2, yes);
+    tile(t + 3, s3, yes);
+  }
+  for (;;) {
+    if (!tile(t++, s0, no)) break;
+    if (!tile(t++, s1, no)) break;
+    if (!tile(t++, s2, no)) break;
+    if (!tile(t++, s3, no)) break;
+  }
   landed(s0);   // no wave reads codes any more
 
   // Element e of lane (r, h) of a 32x32 tile: column r, row 8 (e / 4) + 4 h + e % 4. 32 rows of C go through the
   // wave's part of LDS at a time, 16 bytes apart from a multiple of the banks.
   constexpr int ROW = 32 * TN * (int)sizeof(OutT), PITCH = ROW + 16;
   constexpr int LANES = ROW / 16, ROWS = 64 / LANES;   // of a store
-  static_assert(32 * PITCH <= tile_lds(BM, BN) / 4, "a wave's part of LDS");
-  uint8_t* const mine = lds + wave * (tile_lds(BM, BN) / 4);
+  static_assert(32 * PITCH <= tile_lds(BM, BN, STAGES) / 4, "a wave's part of LDS");
+  uint8_t* const mine = lds + wave * (tile_lds(BM, BN, STAGES) / 4);
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -550,41 +593,45 @@ static int sliced(size_t items, const char* what, F launch) {
   return 0;
 }
 
-// The size of the tiles, in rows and columns: 0 for the small kernel, which takes everything.
+// The size of the tiles, in rows and columns: 0 for the small kernel, which takes everything. A round of 256 tiles,
+// one for each CU, takes about 5, 13 and 42 us at K = 4096 for tiles of 64, 128 and 256 (2048x1024: 10.6 against
+// 12.4 us; 2048x2048: 17.5 and 12.7; 3000x3000: 42 and 38; 4096x4096: 74, 51 and 42), in that proportion at any K.
 static int tile_size(int64_t M, int64_t N, int64_t nb) {
-  const int64_t least = M < N ? M : N, cus = 256;
+  const int64_t least = M < N ? M : N;
   if (least < 64 || nb < 8 || nb > 1 << 20) return 0;   // whole tiles inside C, 8 blocks to read, 32-bit offsets in a tile
-  auto tiles = [&](int64_t b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
-  if (least >= 256 && tiles(256) >= cus) return 256;
-  if (least >= 128 && tiles(128) >= cus) return 128;
-  return 64;
+  auto rounds = [&](int64_t b) { return (((M + b - 1) / b) * ((N + b - 1) / b) + 255) / 256; };
+  int best = 64;
+  int64_t cost = rounds(64) * 5;
+  if (least >= 128 && rounds(128) * 13 < cost) best = 128, cost = rounds(128) * 13;
+  if (least >= 256 && rounds(256) * 42 < cost) best = 256;
+  return best;
 }
 
 static int64_t arranged_bytes(int64_t M, int64_t N, int64_t nb) {
   return ((M + 255) / 256 + (N + 255) / 256) * 2 * ((nb + 7) / 8) * 1024;
 }
 
-template <typename OutT, int T>
+template <typename OutT, int T, int STAGES>
 static int launch_tile(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
                        int64_t nb, float alpha, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-  constexpr int BM = 64 * T, LDS = tile_lds(BM, BM);
+  constexpr int BM = 64 * T, LDS = tile_lds(BM, BM, STAGES);
   constexpr bool ARRANGED = T == 4;
   if (M < BM || N < BM || nb < 8 || nb > 1 << 20)   // what the kernel's addresses assume
     return kamd_fail("gemm_mxfp4_nt: no tile of %d in %lld x %lld x %lld blocks", BM, (long long)M, (long long)N, (long long)nb);
   const int64_t tiles = ((M + BM - 1) / BM) * ((N + BM - 1) / BM);
   if (tiles >= (int64_t)1 << 24) return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)M, (long long)N);
-  auto kernel = gemm_tile_kernel<OutT, T, T, ARRANGED>;
+  auto kernel = gemm_tile_kernel<OutT, T, T, STAGES, ARRANGED>;
   if (ARRANGED) {
     if (!workspace || workspace_bytes < arranged_bytes(M, N, nb) || ((uintptr_t)workspace & 15))
       return kamd_fail("gemm_mxfp4_nt: needs a workspace of %lld bytes, 16-byte aligned", (long long)arranged_bytes(M, N, nb));
-    // more than 64 KiB of LDS has to be asked for, on every device that the kernel runs on
-    if (LDS > 64 * 1024) HC(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
     const int64_t panels = ((M + 255) / 256 + (N + 255) / 256) * 2;
-    hipLaunchKernelGGL(arrange_scales_kernel, dim3((unsigned)panels, (unsigned)((nb + 31) / 32)), dim3(256), 0, stream,
+    hipLaunchKernelGGL(arrange_scales_kernel, dim3((unsigned)panels, (unsigned)((nb + 63) / 64)), dim3(256), 0, stream,
                        (const uint8_t*)As, (const uint8_t*)Bs, (uint8_t*)workspace, (int)M, (int)N, (int)nb);
     HC(hipGetLastError());
     As = workspace;
   }
+  // more than 64 KiB of LDS has to be asked for, on every device that the kernel runs on
+  if (LDS > 64 * 1024) HC(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
   hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), LDS, stream, (const uint8_t*)A, (const uint8_t*)As,
                      (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, alpha);
   return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
@@ -600,9 +647,13 @@ static int launch_gemm(const void* A, const void* As, const void* B, const void*
     return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
   }
   switch (tile_size(M, N, nb)) {
-    case 256: return launch_tile<OutT, 4>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);
-    case 128: return launch_tile<OutT, 2>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream);
-    case 64: return launch_tile<OutT, 1>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream);
+    case 256: return launch_tile<OutT, 4, 2>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);
+    case 128:
+      // one tile a CU: 4 stages; more: 2, and two tiles on a CU (2048x2048x8192: 25 and 30 us, 4096x2048x4096: 32 and 27)
+      return ((M + 127) / 128) * ((N + 127) / 128) <= 256
+                 ? launch_tile<OutT, 2, 4>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream)
+                 : launch_tile<OutT, 2, 2>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream);
+    case 64: return launch_tile<OutT, 1, 4>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream);
   }
   const int64_t tiles = ((M + 15) / 16) * ((N + 15) / 16);
   if (tiles * (SMALL_WAVES * 64) >= (int64_t)1 << 32)
