@@ -14,7 +14,6 @@ rather than silently falling back to a PyTorch implementation.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 
@@ -130,31 +129,47 @@ def gemm_fp8_nt(a, b, out_fp32=True, alpha=1.0):
 
 
 MXFP4_BLOCK = 32
+_mx_type_codes = {}
 
 
 def _mx_types():
-    import torch
-    return {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+    """The C entries' codes of the types that fp4 is made from and turned into."""
+    if not _mx_type_codes:
+        import torch
+        _mx_type_codes.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2})
+    return _mx_type_codes
 
 
-def _on(t):
-    """Launches go to the tensor's device, whichever is current."""
+def _mx_launch(t, what, entry, *args):
+    """A launch on the current stream of the tensor's device, whichever device is current."""
     import torch
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    _raise(rc, what)
 
 
 def _mx_pair(q, scale, what):
-    """Codes and scales as contiguous bytes, `q` 16-byte aligned: views where they are so already."""
+    """Codes and scales as contiguous bytes, `q` 16-byte aligned: as they are where they are so already."""
     import torch
-    if q.dtype not in (torch.uint8, torch.float4_e2m1fn_x2):
+    u8 = torch.uint8
+    if q.dtype not in (u8, torch.float4_e2m1fn_x2):
         raise ValueError(f"{what}: codes must be uint8 or float4_e2m1fn_x2, got {q.dtype}")
-    if scale.dtype not in (torch.uint8, torch.float8_e8m0fnu):
+    if scale.dtype not in (u8, torch.float8_e8m0fnu):
         raise ValueError(f"{what}: scales must be uint8 or float8_e8m0fnu, got {scale.dtype}")
-    if q.dim() < 1 or q.dim() != scale.dim() or q.shape[:-1] != scale.shape[:-1] or q.shape[-1] != 16 * scale.shape[-1]:
-        raise ValueError(f"{what}: codes [..., 16 * blocks] need scales [..., blocks], got {tuple(q.shape)} and {tuple(scale.shape)}")
+    qs, ss = q.shape, scale.shape
+    if not qs or len(qs) != len(ss) or qs[-1] != 16 * ss[-1] or qs[:-1] != ss[:-1]:
+        raise ValueError(f"{what}: codes [..., 16 * blocks] need scales [..., blocks], got {tuple(qs)} and {tuple(ss)}")
     if q.device != scale.device:
         raise ValueError(f"{what}: codes on {q.device}, scales on {scale.device}")
-    q, scale = q.view(torch.uint8).contiguous(), scale.view(torch.uint8).contiguous()
+    if q.dtype is not u8:
+        q = q.view(u8)
+    if scale.dtype is not u8:
+        scale = scale.view(u8)
+    q, scale = q.contiguous(), scale.contiguous()
     return q.clone() if q.data_ptr() % 16 else q, scale
 
 
@@ -172,24 +187,23 @@ def mxfp4_quantize(x):
     most). The lower index is in the low nibble; a last short block is filled with zeros. A block that holds
     a NaN or an infinity gets s = 255: all of it stands for NaN. No gradient is recorded."""
     import torch
-    types = _mx_types()
-    if x.dtype not in types:
+    code = _mx_types().get(x.dtype)
+    if code is None:
         raise ValueError(f"mxfp4_quantize needs bf16, fp16 or fp32, got {x.dtype}")
     if x.dim() < 1:
         raise ValueError("mxfp4_quantize needs at least one dimension")
     _mx_gpu(x, "mxfp4_quantize")
-    K = x.shape[-1]
+    *lead, K = x.shape
     nb = -(-K // MXFP4_BLOCK)
-    q = torch.empty((*x.shape[:-1], 16 * nb), device=x.device, dtype=torch.uint8)
-    scale = torch.empty((*x.shape[:-1], nb), device=x.device, dtype=torch.uint8)
+    q = torch.empty((*lead, 16 * nb), device=x.device, dtype=torch.uint8)
+    scale = torch.empty((*lead, nb), device=x.device, dtype=torch.uint8)
     if x.numel() == 0:
         return q, scale
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
-    if x2.stride(1) != 1 and K > 1:
+    x2 = x if len(lead) == 1 else x.reshape(-1, K)
+    if K > 1 and x2.stride(1) != 1:
         x2 = x2.contiguous()
-    with _on(x):
-        _raise(load().kamd_mxfp4_quantize_launch(x2.data_ptr(), q.data_ptr(), scale.data_ptr(), x2.shape[0], K,
-                                                 x2.stride(0), types[x.dtype], _stream(x)), "mxfp4_quantize")
+    _mx_launch(x2, "mxfp4_quantize", load().kamd_mxfp4_quantize_launch, x2.data_ptr(), q.data_ptr(), scale.data_ptr(),
+               x2.shape[0], K, x2.stride(0), code)
     return q, scale
 
 
@@ -198,29 +212,28 @@ def mxfp4_dequantize(q, scale, k=None, dtype=None):
     once to `dtype` (bf16 unless given; fp16, fp32). `k` leaves out what fills the last block; 32 * nb unless
     given. Scale 255 gives NaN. Codes and scales are uint8 or torch's float4_e2m1fn_x2 and float8_e8m0fnu."""
     import torch
-    types = _mx_types()
     dtype = torch.bfloat16 if dtype is None else dtype
-    if dtype not in types:
+    code = _mx_types().get(dtype)
+    if code is None:
         raise ValueError(f"mxfp4_dequantize gives bf16, fp16 or fp32, not {dtype}")
     q, scale = _mx_pair(q, scale, "mxfp4_dequantize")
-    nb = scale.shape[-1]
+    *lead, nb = scale.shape
     k = MXFP4_BLOCK * nb if k is None else int(k)
-    if -(-k // MXFP4_BLOCK) != nb or k < 0:
+    if k < 0 or -(-k // MXFP4_BLOCK) != nb:
         raise ValueError(f"mxfp4_dequantize: k={k} does not have {nb} blocks of {MXFP4_BLOCK}")
     _mx_gpu(q, "mxfp4_dequantize")
-    x = torch.empty((*q.shape[:-1], k), device=q.device, dtype=dtype)
+    x = torch.empty((*lead, k), device=q.device, dtype=dtype)
     if x.numel() == 0:
         return x
-    with _on(q):
-        _raise(load().kamd_mxfp4_dequantize_launch(q.data_ptr(), scale.data_ptr(), x.data_ptr(), x.numel() // k, k,
-                                                   types[dtype], _stream(q)), "mxfp4_dequantize")
+    _mx_launch(q, "mxfp4_dequantize", load().kamd_mxfp4_dequantize_launch, q.data_ptr(), scale.data_ptr(), x.data_ptr(),
+               scale.numel() // nb, k, code)
     return x
 
 
 def gemm_mxfp4_nt(a, a_scale, b, b_scale, out_fp32=True, alpha=1.0):
     """C = alpha * a @ b.T of microscaled fp4 operands as mxfp4_quantize makes them: a [M, 16 * nb], a_scale
     [M, nb], b [N, 16 * nb], b_scale [N, nb]; sums in fp32, C fp32 or bf16. Any M and N; K is 32 * nb. A block
-    of scale 255 makes every output that it enters NaN."""
+    of scale 255 makes every output that it enters NaN. No gradient is recorded."""
     import torch
     if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1]:
         raise ValueError(f"gemm_mxfp4_nt needs codes [M, 16 * blocks] and [N, 16 * blocks], got {tuple(a.shape)} and {tuple(b.shape)}")
@@ -229,14 +242,14 @@ def gemm_mxfp4_nt(a, a_scale, b, b_scale, out_fp32=True, alpha=1.0):
     a, a_scale = _mx_pair(a, a_scale, "gemm_mxfp4_nt a")
     b, b_scale = _mx_pair(b, b_scale, "gemm_mxfp4_nt b")
     _mx_gpu(a, "gemm_mxfp4_nt")
-    M, N, nb = a.shape[0], b.shape[0], a_scale.shape[1]
+    (M, nb), N = a_scale.shape, b.shape[0]
+    L = load()
     out = torch.empty((M, N), device=a.device, dtype=torch.float32 if out_fp32 else torch.bfloat16)
-    need = load().kamd_gemm_mxfp4_nt_workspace(M, N, nb)
+    need = L.kamd_gemm_mxfp4_nt_workspace(M, N, nb)
     ws = torch.empty(need, device=a.device, dtype=torch.uint8) if need else None
-    with _on(a):
-        _raise(load().kamd_gemm_mxfp4_nt_launch(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(),
-                                                out.data_ptr(), M, N, nb, float(alpha), 1 if out_fp32 else 0,
-                                                ws.data_ptr() if need else None, need, _stream(a)), "gemm_mxfp4_nt")
+    _mx_launch(a, "gemm_mxfp4_nt", L.kamd_gemm_mxfp4_nt_launch, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
+               b_scale.data_ptr(), out.data_ptr(), M, N, nb, float(alpha), 1 if out_fp32 else 0,
+               ws.data_ptr() if need else None, need)
     return out
 
 

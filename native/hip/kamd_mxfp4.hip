@@ -184,43 +184,6 @@ __device__ __forceinline__ i32x8 frag(i32x4 v) { return i32x8{v.x, v.y, v.z, v.w
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__bf16* p, float v) { *p = (__bf16)v; }
 
-// One 16x16 tile a workgroup; its 4 waves take the steps of K in turn and join their sums in LDS.
-// Rows behind the last are read as the last row and not stored. Chunks behind the last block are read as
-// the row's last block, with their codes cleared and the scale set to 1 on both sides.
-constexpr int SMALL_WAVES = 4;
-template <typename OutT>
-__global__ void __launch_bounds__(SMALL_WAVES * 64)
-gemm_small_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, const uint8_t* __restrict__ B,
-                  const uint8_t* __restrict__ Bs, OutT* __restrict__ C, int M, int N, int nb, float alpha) {
-  __shared__ f32x4 part[SMALL_WAVES][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r = lane & 15, g = lane >> 4;
-  const int tiles_n = (N + 15) / 16;
-  const int m0 = (int)(blockIdx.x / tiles_n) * 16, n0 = (int)(blockIdx.x % tiles_n) * 16;
-  const size_t ra = (size_t)min(m0 + r, M - 1) * nb, rb = (size_t)min(n0 + r, N - 1) * nb;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int c0 = wave * 4; c0 < nb; c0 += SMALL_WAVES * 4) {
-    const int c = min(c0 + g, nb - 1);
-    i32x4 a = *(const i32x4*)(A + (ra + c) * 16), b = *(const i32x4*)(B + (rb + c) * 16);
-    int sa = As[ra + c], sb = Bs[rb + c];
-    if (c0 + g >= nb) {
-      a = b = i32x4{0, 0, 0, 0};
-      sa = sb = 127;
-    }
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(frag(a), frag(b), acc, 4, 4, 0, sa, 0, sb);
-  }
-  part[wave][lane] = acc;
-  __syncthreads();
-  if (wave != 0) return;
-#pragma unroll
-  for (int w = 1; w < SMALL_WAVES; ++w) acc += part[w][lane];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = m0 + g * 4 + j, col = n0 + r;
-    if (row < M && col < N) store_out(C + (size_t)row * N + col, alpha * acc[j]);
-  }
-}
-
 template <typename OutT>
 __global__ void __launch_bounds__(256) zero_kernel(OutT* __restrict__ C, size_t n) {
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -579,6 +542,137 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   }
 }
 
+// Products of few rows, whose time is the reading of the other operand. P is the operand with the many rows, Q that
+// with the few; a workgroup makes NP x NQ tiles of 16x16 (v_mfma_scale_f32_16x16x128_f8f6f4), its WAVES taking units
+// of 8 blocks (256 values, 128 B a row) of K in turn, each through two buffers of its own in LDS: no wave waits for
+// another before the sums meet, in the order of the waves. (Straight to registers the instruction's layout has
+// neighbouring lanes read different rows, 16 bytes of each: 32x8192x8192 took 13.3 us so.) Slots in LDS, and what is
+// read behind the last row and block, are as in the tiles above; lane (r, g) takes chunks 2 g and 2 g + 1 of row r,
+// whose scales are one 16-bit word, the instruction's byte select taking them apart.
+constexpr int rows_lds(int NP, int NQ, int WAVES) { return WAVES * 2 * (NP + NQ) * 16 * 128; }
+
+template <typename OutT, int NP, int NQ, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64)
+gemm_rows_kernel(const uint8_t* __restrict__ P, const uint8_t* __restrict__ Ps, const uint8_t* __restrict__ Q,
+                 const uint8_t* __restrict__ Qs, OutT* __restrict__ C, int np, int nq, int nb, int64_t cp, int64_t cq,
+                 float alpha) {
+  constexpr int GROUPS = NP + NQ, UNIT = GROUPS * 16 * 128, LOADS = GROUPS * 2;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int tiles_p = (np + NP * 16 - 1) / (NP * 16);
+  const int p0 = (int)(blockIdx.x % tiles_p) * NP * 16, q0 = (int)(blockIdx.x / tiles_p) * NQ * 16;
+  const int units = nb / 8, rem = nb % 8;   // whole units, blocks of a short one
+  uint8_t* const mine = lds + wave * 2 * UNIT;
+
+  // the block that row i starts with of the 16 GROUPS
+  auto row = [&](int i) { return (size_t)(i < NP * 16 ? min(p0 + i, np - 1) : min(q0 + i - NP * 16, nq - 1)) * nb; };
+  size_t from[LOADS];   // a load takes 8 rows of 128 B
+  const int chunk[2] = {(lane & 7) ^ (lane >> 4), (lane & 7) ^ (4 + (lane >> 4))};   // of even loads, of odd ones
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) from[j] = (row(j * 8 + (lane >> 3)) + chunk[j % 2]) * 16;
+  size_t srow[GROUPS];
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) srow[i] = row(i * 16 + r);
+
+  struct Scales { uint32_t v[GROUPS]; };
+  auto load = [&](int t, int buffer, Scales& s, auto part) {
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+      const uint8_t* p = (i < NP ? Ps : Qs) + srow[i] + (size_t)t * 8 + g * 2;
+      if (part) {   // 1 behind the last block
+        s.v[i] = (g * 2 < rem ? p[0] : 127) | (g * 2 + 1 < rem ? p[1] : 127) << 8;
+      } else {
+        uint16_t v;
+        __builtin_memcpy(&v, p, 2);
+        s.v[i] = v;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const uint8_t* p = (j < NP * 2 ? P : Q) + from[j] + (size_t)t * 128;
+      if (part && chunk[j % 2] >= rem) p -= (chunk[j % 2] - rem + 1) * 16;
+      __builtin_amdgcn_global_load_lds((const void*)p, (lds_void*)(mine + buffer * UNIT + j * 1024), 16, 0, 0);
+    }
+  };
+  f32x4 acc[NP][NQ];
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](int buffer, const Scales& s, auto part) {
+    unroll<2>([&](auto k) {
+      i32x4 v[GROUPS];
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i)
+        v[i] = *(const i32x4*)(mine + buffer * UNIT + (i * 16 + r) * 128 + (((2 * g + k) ^ (r >> 1)) << 4));
+      if (part && 2 * g + k >= rem) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) v[NP + j] = i32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(frag(v[i]), frag(v[NP + j]), acc[i][j], 4, 4, k,
+                                                                        (int)s.v[i], k, (int)s.v[NP + j]);
+    });
+  };
+  auto arrived = [](auto keep) {   // all but the last of this wave's loads
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(waitcnt(keep, 15));
+    asm volatile("" ::: "memory");
+  };
+  constexpr std::integral_constant<int, 0> none{};
+  constexpr std::false_type whole{};
+  constexpr std::true_type part{};
+  // unit t in one buffer, the wave's next on its way into the other, whose last reads have returned
+  Scales s[2];
+  auto unit = [&](int t, auto buffer) {
+    const bool more = t + WAVES < units;
+    if (more) {
+      load(t + WAVES, 1 - buffer, s[1 - buffer], whole);
+      arrived(std::integral_constant<int, LOADS>{});
+      multiply(buffer, s[buffer], whole);
+    } else {
+      arrived(none);
+      multiply(buffer, s[buffer], whole);
+    }
+    return more;
+  };
+  int t = wave;
+  if (t < units) {
+    load(t, 0, s[0], whole);
+    for (;; t += 2 * WAVES) {
+      if (!unit(t, none)) break;
+      if (!unit(t + WAVES, std::integral_constant<int, 1>{})) break;
+    }
+  }
+  if (rem && wave == units % WAVES) {
+    load(units, 0, s[0], part);
+    arrived(none);
+    multiply(0, s[0], part);
+  }
+  __syncthreads();
+  f32x4* const sums = (f32x4*)lds;   // [WAVES][NP * NQ][64]
+  static_assert(WAVES * NP * NQ * 1024 <= rows_lds(NP, NQ, WAVES), "the sums' place");
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) sums[(wave * NP * NQ + i * NQ + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  for (int k = wave; k < NP * NQ; k += WAVES) {
+    f32x4 sum = sums[k * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) sum += sums[(w * NP * NQ + k) * 64 + lane];
+    const int p = p0 + k / NQ * 16 + g * 4, q = q0 + k % NQ * 16 + r;
+    if (q >= nq) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (p + e < np) store_out(C + (p + e) * cp + q * cq, alpha * sum[e]);
+  }
+}
+
 // A launch's workgroups times 256 lanes stay below 2^32; longer runs take several launches.
 constexpr size_t SLICE = (size_t)1 << 31;
 
@@ -594,8 +688,9 @@ static int sliced(size_t items, const char* what, F launch) {
 }
 
 // The size of the tiles, in rows and columns: 0 for the small kernel, which takes everything. A round of 256 tiles,
-// one for each CU, takes about 5, 13 and 42 us at K = 4096 for tiles of 64, 128 and 256 (2048x1024: 10.6 against
-// 12.4 us; 2048x2048: 17.5 and 12.7; 3000x3000: 42 and 38; 4096x4096: 74, 51 and 42), in that proportion at any K.
+// one for each CU, takes about 5 and 13 us at K = 4096 for tiles of 64 and 128, and 28 to 42 for 256, whose full rounds
+// run into the power limit (2048x1024: 10.6 against 12.4 us; 2048x2048: 17.5 and 12.7; 4096x2560: 48, 38 and 34;
+// 4096x4096: 74, 51 and 42), in that proportion at any K.
 static int tile_size(int64_t M, int64_t N, int64_t nb) {
   const int64_t least = M < N ? M : N;
   if (least < 64 || nb < 8 || nb > 1 << 20) return 0;   // whole tiles inside C, 8 blocks to read, 32-bit offsets in a tile
@@ -603,7 +698,8 @@ static int tile_size(int64_t M, int64_t N, int64_t nb) {
   int best = 64;
   int64_t cost = rounds(64) * 5;
   if (least >= 128 && rounds(128) * 13 < cost) best = 128, cost = rounds(128) * 13;
-  if (least >= 256 && rounds(256) * 42 < cost) best = 256;
+  const int64_t tiles256 = ((M + 255) / 256) * ((N + 255) / 256);
+  if (least >= 256 && rounds(256) * 28 + tiles256 * 14 / 256 < cost) best = 256;
   return best;
 }
 
@@ -637,6 +733,42 @@ static int launch_tile(const void* A, const void* As, const void* B, const void*
   return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
 }
 
+template <typename OutT, int NP, int NQ, int WAVES>
+static int launch_rows_of(const void* P, const void* Ps, const void* Q, const void* Qs, void* C, int64_t np, int64_t nq,
+                          int64_t nb, int64_t cp, int64_t cq, float alpha, hipStream_t stream) {
+  constexpr int LDS = rows_lds(NP, NQ, WAVES);
+  const int64_t tiles = ((np + NP * 16 - 1) / (NP * 16)) * ((nq + NQ * 16 - 1) / (NQ * 16));
+  if (tiles * (WAVES * 64) >= (int64_t)1 << 32) return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)np, (long long)nq);
+  auto kernel = gemm_rows_kernel<OutT, NP, NQ, WAVES>;
+  if (LDS > 64 * 1024) HC(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(WAVES * 64), LDS, stream, (const uint8_t*)P, (const uint8_t*)Ps,
+                     (const uint8_t*)Q, (const uint8_t*)Qs, (OutT*)C, (int)np, (int)nq, (int)nb, cp, cq, alpha);
+  return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
+}
+
+template <typename OutT>
+static int launch_rows(const void* P, const void* Ps, const void* Q, const void* Qs, void* C, int64_t np, int64_t nq, int64_t nb,
+                       int64_t cp, int64_t cq, float alpha, hipStream_t stream) {
+  // Two tiles of P where one would make more than a workgroup for each CU: half the reads of Q, and one round
+  // (16x5000x4096: 4.7 against 5.0 us, 32x5000x4096: 5.8 and 7.9). Eight waves where the workgroups are one for each
+  // CU, whose LDS they fill; of more, with four, two lie on a CU (32x8192x8192: 8.9 against 10.0 us with four;
+  // 32x10000x4096: 10.3 with eight and 8.8).
+  const int64_t cus = 256, each = (nq + 15) / 16;
+  const bool wide = np > 16 * cus;
+  const bool many = (np + (wide ? 31 : 15)) / (wide ? 32 : 16) * (each <= 2 ? 1 : (each + 3) / 4) > cus;
+#define KAMD_ROWS(NP, NQ, W) launch_rows_of<OutT, NP, NQ, W>(P, Ps, Q, Qs, C, np, nq, nb, cp, cq, alpha, stream)
+  if (each == 1) {
+    if (wide) return many ? KAMD_ROWS(2, 1, 4) : KAMD_ROWS(2, 1, 8);
+    return KAMD_ROWS(1, 1, 8);
+  }
+  if (each == 2) {
+    if (wide) return many ? KAMD_ROWS(2, 2, 4) : KAMD_ROWS(2, 2, 8);
+    return KAMD_ROWS(1, 2, 8);
+  }
+  return wide ? KAMD_ROWS(2, 4, 4) : KAMD_ROWS(1, 4, 4);
+#undef KAMD_ROWS
+}
+
 template <typename OutT>
 static int launch_gemm(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N, int64_t nb,
                        float alpha, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
@@ -655,12 +787,9 @@ static int launch_gemm(const void* A, const void* As, const void* B, const void*
                  : launch_tile<OutT, 2, 2>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream);
     case 64: return launch_tile<OutT, 1, 4>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream);
   }
-  const int64_t tiles = ((M + 15) / 16) * ((N + 15) / 16);
-  if (tiles * (SMALL_WAVES * 64) >= (int64_t)1 << 32)
-    return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)M, (long long)N);
-  hipLaunchKernelGGL(gemm_small_kernel<OutT>, dim3((unsigned)tiles), dim3(SMALL_WAVES * 64), 0, stream, (const uint8_t*)A,
-                     (const uint8_t*)As, (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, alpha);
-  return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
+  // the operand with more rows is P; element (p, q) of the product at p * cp + q * cq
+  return M <= N ? launch_rows<OutT>(B, Bs, A, As, C, N, M, nb, 1, N, alpha, stream)
+                : launch_rows<OutT>(A, As, B, Bs, C, M, N, nb, N, 1, alpha, stream);
 }
 }  // namespace mxfp4
 
