@@ -43,7 +43,7 @@ def load():
         L.kamd_gemm_bf16_nt_launch.argtypes = [vp, vp, vp, i, i, i, i, f, i, vp]
         L.kamd_gemm_fp8_nt_launch.argtypes = [vp, vp, vp, i, i, i, i, f, i, vp]
         i64 = ctypes.c_int64
-        L.kamd_mxfp4_quantize_launch.argtypes = [vp, vp, vp, i64, i64, i64, i, vp]
+        L.kamd_mxfp4_quantize_launch.argtypes = [vp, vp, vp, i64, i64, i64, i64, i, vp]
         L.kamd_mxfp4_dequantize_launch.argtypes = [vp, vp, vp, i64, i64, i, vp]
         L.kamd_gemm_mxfp4_nt_launch.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, f, i, vp, i64, vp]
         L.kamd_gemm_mxfp4_nt_workspace.argtypes = [i64, i64, i64]
@@ -156,11 +156,14 @@ def _mx_pair(q, scale, what):
     """Codes and scales as contiguous bytes, `q` 16-byte aligned: as they are where they are so already."""
     import torch
     u8 = torch.uint8
+    qs, ss = q.shape, scale.shape
+    if (len(qs) == 2 == len(ss) and q.dtype is u8 is scale.dtype and qs[0] == ss[0] and qs[1] == 16 * ss[1]
+            and q.is_contiguous() and scale.is_contiguous() and q.device == scale.device and not q.data_ptr() % 16):
+        return q, scale
     if q.dtype not in (u8, torch.float4_e2m1fn_x2):
         raise ValueError(f"{what}: codes must be uint8 or float4_e2m1fn_x2, got {q.dtype}")
     if scale.dtype not in (u8, torch.float8_e8m0fnu):
         raise ValueError(f"{what}: scales must be uint8 or float8_e8m0fnu, got {scale.dtype}")
-    qs, ss = q.shape, scale.shape
     if not qs or len(qs) != len(ss) or qs[-1] != 16 * ss[-1] or qs[:-1] != ss[:-1]:
         raise ValueError(f"{what}: codes [..., 16 * blocks] need scales [..., blocks], got {tuple(qs)} and {tuple(ss)}")
     if q.device != scale.device:
@@ -195,15 +198,18 @@ def mxfp4_quantize(x):
     _mx_gpu(x, "mxfp4_quantize")
     *lead, K = x.shape
     nb = -(-K // MXFP4_BLOCK)
-    q = torch.empty((*lead, 16 * nb), device=x.device, dtype=torch.uint8)
-    scale = torch.empty((*lead, nb), device=x.device, dtype=torch.uint8)
-    if x.numel() == 0:
+    dev, u8 = x.device, torch.uint8
+    q = torch.empty((*lead, 16 * nb), device=dev, dtype=u8)
+    scale = torch.empty((*lead, nb), device=dev, dtype=u8)
+    if K == 0 or 0 in lead:
         return q, scale
     x2 = x if len(lead) == 1 else x.reshape(-1, K)
-    if K > 1 and x2.stride(1) != 1:
+    row_step, step = x2.stride()
+    if K > 1 and step != 1 and row_step != 1:   # neither rows nor columns in one piece each
         x2 = x2.contiguous()
+        row_step, step = K, 1
     _mx_launch(x2, "mxfp4_quantize", load().kamd_mxfp4_quantize_launch, x2.data_ptr(), q.data_ptr(), scale.data_ptr(),
-               x2.shape[0], K, x2.stride(0), code)
+               x2.shape[0], K, row_step, step, code)
     return q, scale
 
 
@@ -235,17 +241,18 @@ def gemm_mxfp4_nt(a, a_scale, b, b_scale, out_fp32=True, alpha=1.0):
     [M, nb], b [N, 16 * nb], b_scale [N, nb]; sums in fp32, C fp32 or bf16. Any M and N; K is 32 * nb. A block
     of scale 255 makes every output that it enters NaN. No gradient is recorded."""
     import torch
-    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1]:
-        raise ValueError(f"gemm_mxfp4_nt needs codes [M, 16 * blocks] and [N, 16 * blocks], got {tuple(a.shape)} and {tuple(b.shape)}")
+    sa, sb = a.shape, b.shape
+    if len(sa) != 2 or len(sb) != 2 or sa[1] != sb[1]:
+        raise ValueError(f"gemm_mxfp4_nt needs codes [M, 16 * blocks] and [N, 16 * blocks], got {tuple(sa)} and {tuple(sb)}")
     if a.device != b.device:
         raise ValueError(f"gemm_mxfp4_nt: a on {a.device}, b on {b.device}")
     a, a_scale = _mx_pair(a, a_scale, "gemm_mxfp4_nt a")
     b, b_scale = _mx_pair(b, b_scale, "gemm_mxfp4_nt b")
     _mx_gpu(a, "gemm_mxfp4_nt")
-    (M, nb), N = a_scale.shape, b.shape[0]
+    M, N, nb = sa[0], sb[0], sa[1] // 16
     L = load()
     out = torch.empty((M, N), device=a.device, dtype=torch.float32 if out_fp32 else torch.bfloat16)
-    need = L.kamd_gemm_mxfp4_nt_workspace(M, N, nb)
+    need = L.kamd_gemm_mxfp4_nt_workspace(M, N, nb) if M > 16 and N > 16 else 0   # none for a few rows
     ws = torch.empty(need, device=a.device, dtype=torch.uint8) if need else None
     _mx_launch(a, "gemm_mxfp4_nt", L.kamd_gemm_mxfp4_nt_launch, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
                b_scale.data_ptr(), out.data_ptr(), M, N, nb, float(alpha), 1 if out_fp32 else 0,

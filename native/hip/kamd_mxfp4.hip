@@ -10,6 +10,7 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <atomic>
 #include <new>
 #include <type_traits>
 #include <utility>
@@ -64,6 +65,12 @@ template <> struct Oct<FP32> {
     return c;
   }
 };
+// |x| of a 16-bit type as the bits of an fp32
+template <int TYPE>
+__device__ __forceinline__ uint32_t widen(uint32_t v) {
+  if constexpr (TYPE == BF16) return v << 16;
+  else return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)v));
+}
 struct Oct16 {
   uint32_t v[4];   // pairs
   __device__ uint32_t amax16() const {
@@ -74,7 +81,7 @@ struct Oct16 {
   }
 };
 template <> struct Oct<BF16> : Oct16 {
-  __device__ uint32_t amax() const { return amax16() << 16; }
+  __device__ uint32_t amax() const { return widen<BF16>(amax16()); }
   __device__ uint32_t codes(float scale) const {
     uint32_t c = 0;
     c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, v[0]), scale, 0);
@@ -85,9 +92,7 @@ template <> struct Oct<BF16> : Oct16 {
   }
 };
 template <> struct Oct<FP16> : Oct16 {
-  __device__ uint32_t amax() const {
-    return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)amax16()));
-  }
+  __device__ uint32_t amax() const { return widen<FP16>(amax16()); }
   __device__ uint32_t codes(float scale) const {
     uint32_t c = 0;
     c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, v[0]), scale, 0);
@@ -132,6 +137,91 @@ quantize_rows_kernel(const void* __restrict__ xv, uint32_t* __restrict__ q, uint
   const uint32_t s = scale_byte(m);
   q[i] = s == 255 ? 0u : o.codes(__uint_as_float(s << 23));
   if ((threadIdx.x & 3) == 0) scale[i >> 2] = (uint8_t)s;
+}
+
+// The same of x whose columns lie in one piece each (a transposed view): value k of row m at x[k * ld + m]. A wave
+// reads 32 rows of memory, 256 bytes of each, a lane having all 32 values of COLS blocks; 8 blocks of a row go
+// through LDS, so that whole cache lines are written. Rows of memory and columns behind the last read as 0.
+template <int TYPE>
+__global__ void __launch_bounds__(256)
+quantize_cols_kernel(const void* __restrict__ xv, uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int64_t M, int64_t K,
+                     int64_t ld, int64_t nb) {
+  typedef typename Elem<TYPE>::bits bits;
+  constexpr int COLS = TYPE == FP32 ? 1 : 2, ROWS = 64 * COLS, PITCH = 128 + 16;
+  __shared__ __attribute__((aligned(16))) uint8_t codes[ROWS * PITCH];
+  __shared__ __attribute__((aligned(8))) uint8_t scales[ROWS * 8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t tiles_m = (M + ROWS - 1) / ROWS;
+  const int64_t m0 = (int64_t)blockIdx.x % tiles_m * ROWS, b0 = (int64_t)blockIdx.x / tiles_m * 8;
+  const int64_t m = m0 + lane * COLS;
+  for (int b = wave * 2; b < wave * 2 + 2; ++b) {
+    const int64_t k0 = (b0 + b) * 32;
+    const bits* p = (const bits*)xv + k0 * ld + m;
+    uint32_t v[32];
+    const int ks = (int)(K - k0 < 32 ? K - k0 : 32);   // <= 0: no block
+    if (ks == 32 && m + COLS <= M) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) __builtin_memcpy(&v[k], p + k * ld, 4);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        v[k] = 0;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+          if (k < ks && m + c < M) v[k] |= (uint32_t)p[k * ld + c] << (16 * c);
+      }
+    }
+    // each column's codes as those of 4 lanes of the kernel above
+    uint32_t amax[COLS];
+    if constexpr (TYPE == FP32) {
+      amax[0] = 0;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) amax[0] = max(amax[0], v[k] & 0x7fffffffu);
+    } else {
+      u16x2 a = {0, 0};
+#pragma unroll
+      for (int k = 0; k < 32; ++k) a = __builtin_elementwise_max(a, __builtin_bit_cast(u16x2, v[k] & 0x7fff7fffu));
+      amax[0] = widen<TYPE>(a.x);
+      amax[1] = widen<TYPE>(a.y);
+    }
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      const uint32_t s = scale_byte(amax[c]);
+      uint32_t out[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        Oct<TYPE> o;
+        if constexpr (TYPE == FP32) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o.v[k] = v[i * 8 + k];
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            o.v[k] = __builtin_amdgcn_perm(v[i * 8 + k * 2 + 1], v[i * 8 + k * 2], c == 0 ? 0x05040100u : 0x07060302u);
+        }
+        out[i] = s == 255 ? 0u : o.codes(__uint_as_float(s << 23));
+      }
+      __builtin_memcpy(__builtin_assume_aligned(codes + (lane * COLS + c) * PITCH + b * 16, 16), out, 16);
+      scales[(lane * COLS + c) * 8 + b] = (uint8_t)s;
+    }
+  }
+  __syncthreads();
+  const int blocks = (int)(nb - b0 < 8 ? nb - b0 : 8);
+#pragma unroll
+  for (int i = 0; i < ROWS / 32; ++i) {
+    const int row = i * 32 + tid / 8, b = tid % 8;
+    if (m0 + row >= M || b >= blocks) continue;
+    const i32x4 v = *(const i32x4*)(codes + row * PITCH + b * 16);
+    *((i32x4*)q + (m0 + row) * nb + b0 + b) = v;
+  }
+  if (tid < ROWS && m0 + tid < M) {
+    uint8_t* p = scale + (m0 + tid) * nb + b0;
+    if (blocks == 8) {
+      __builtin_memcpy(p, __builtin_assume_aligned(scales + tid * 8, 8), 8);
+    } else {
+      for (int b = 0; b < blocks; ++b) p[b] = scales[tid * 8 + b];
+    }
+  }
 }
 
 // The inverse, rounded once to the output's type. v_cvt_scalef32_pk_*_fp4 gives NaN for s = 255.
@@ -707,6 +797,19 @@ static int64_t arranged_bytes(int64_t M, int64_t N, int64_t nb) {
   return ((M + 255) / 256 + (N + 255) / 256) * 2 * ((nb + 7) / 8) * 1024;
 }
 
+// More than 64 KiB of LDS has to be asked for, once on every device that the kernel runs on.
+template <typename F>
+static int allow_lds(F kernel, int bytes, std::atomic<uint64_t>& asked) {
+  if (bytes <= 64 * 1024) return 0;
+  int dev = 0;
+  HC(hipGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if (bit && (asked.load(std::memory_order_relaxed) & bit)) return 0;
+  HC(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  asked.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
+}
+
 template <typename OutT, int T, int STAGES>
 static int launch_tile(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
                        int64_t nb, float alpha, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
@@ -726,8 +829,8 @@ static int launch_tile(const void* A, const void* As, const void* B, const void*
     HC(hipGetLastError());
     As = workspace;
   }
-  // more than 64 KiB of LDS has to be asked for, on every device that the kernel runs on
-  if (LDS > 64 * 1024) HC(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+  static std::atomic<uint64_t> asked{0};
+  if (allow_lds(kernel, LDS, asked) != 0) return -1;
   hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), LDS, stream, (const uint8_t*)A, (const uint8_t*)As,
                      (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, alpha);
   return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
@@ -740,7 +843,8 @@ static int launch_rows_of(const void* P, const void* Ps, const void* Q, const vo
   const int64_t tiles = ((np + NP * 16 - 1) / (NP * 16)) * ((nq + NQ * 16 - 1) / (NQ * 16));
   if (tiles * (WAVES * 64) >= (int64_t)1 << 32) return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)np, (long long)nq);
   auto kernel = gemm_rows_kernel<OutT, NP, NQ, WAVES>;
-  if (LDS > 64 * 1024) HC(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+  static std::atomic<uint64_t> asked{0};
+  if (allow_lds(kernel, LDS, asked) != 0) return -1;
   hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(WAVES * 64), LDS, stream, (const uint8_t*)P, (const uint8_t*)Ps,
                      (const uint8_t*)Q, (const uint8_t*)Qs, (OutT*)C, (int)np, (int)nq, (int)nb, cp, cq, alpha);
   return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
@@ -795,21 +899,29 @@ static int launch_gemm(const void* A, const void* As, const void* B, const void*
 
 extern "C" {
 
-// x: rows of K values (type 0 bf16, 1 fp16, 2 fp32), row r at x + r * ld elements; q: rows * 16 * nb bytes, 4-byte
-// aligned; scale: rows * nb bytes
-int kamd_mxfp4_quantize_launch(const void* x, void* q, void* scale, int64_t rows, int64_t K, int64_t ld, int type,
-                               hipStream_t stream) {
-  if (rows < 0 || K < 0 || type < 0 || type > 2) return kamd_fail("mxfp4_quantize: bad arguments");
+// x: rows of K values (type 0 bf16, 1 fp16, 2 fp32), value k of row r at x + r * row_step + k * step elements, one of the
+// two steps being 1; q: rows * 16 * nb bytes, 16-byte aligned; scale: rows * nb bytes
+int kamd_mxfp4_quantize_launch(const void* x, void* q, void* scale, int64_t rows, int64_t K, int64_t row_step, int64_t step,
+                               int type, hipStream_t stream) {
+  using namespace mxfp4;
+  if (rows < 0 || K < 0 || type < 0 || type > 2 || (step != 1 && row_step != 1 && K > 1))
+    return kamd_fail("mxfp4_quantize: bad arguments");
   if (rows == 0 || K == 0) return 0;
-  const int64_t row_items = (K + 31) / 32 * 4;
+  const int64_t nb = (K + 31) / 32, row_items = nb * 4;
   if (row_items >= (int64_t)1 << 31) return kamd_fail("mxfp4_quantize: K (%lld) is too large", (long long)K);
+  if (((uintptr_t)q) & 15) return kamd_fail("mxfp4_quantize: codes must be 16-byte aligned");
+  if (step != 1 && K > 1) {
+    const int64_t tile = type == FP32 ? 64 : 128, tiles = (rows + tile - 1) / tile * ((nb + 7) / 8);
+    if (tiles >= (int64_t)1 << 24) return kamd_fail("mxfp4_quantize: %lld x %lld is too large", (long long)rows, (long long)K);
+    auto k = type == BF16 ? quantize_cols_kernel<BF16> : type == FP16 ? quantize_cols_kernel<FP16> : quantize_cols_kernel<FP32>;
+    hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(256), 0, stream, x, (uint8_t*)q, (uint8_t*)scale, rows, K, step, nb);
+    return kamd_check(hipGetLastError(), "mxfp4_quantize launch");
+  }
   const size_t items = (size_t)rows * row_items;
-  return mxfp4::sliced(items, "mxfp4_quantize", [&](size_t first, dim3 grid) {
-    auto k = type == mxfp4::BF16   ? mxfp4::quantize_rows_kernel<mxfp4::BF16>
-             : type == mxfp4::FP16 ? mxfp4::quantize_rows_kernel<mxfp4::FP16>
-                                   : mxfp4::quantize_rows_kernel<mxfp4::FP32>;
-    hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, x, (uint32_t*)q, (uint8_t*)scale, first, items,
-                       (uint32_t)row_items, K, ld);
+  return sliced(items, "mxfp4_quantize", [&](size_t first, dim3 grid) {
+    auto k = type == BF16 ? quantize_rows_kernel<BF16> : type == FP16 ? quantize_rows_kernel<FP16> : quantize_rows_kernel<FP32>;
+    hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, x, (uint32_t*)q, (uint8_t*)scale, first, items, (uint32_t)row_items, K,
+                       row_step);
   });
 }
 

@@ -189,13 +189,18 @@ def test_quantize_ties_zeros_and_blocks_without_an_answer(gpu, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,K", [(1, 64), (2, 1), (31, 33), (64, 32), (65, 100), (128, 256), (130, 259), (257, 513), (8, 4097)])
+@pytest.mark.parametrize("rows,K", [(1, 64), (2, 1), (31, 33), (64, 32), (65, 100), (128, 256), (130, 259), (257, 513), (8, 4097),
+                                    (127, 287), (640, 1000)])
 def test_quantize_strides(gpu, dtype, rows, K):
     g = torch.Generator().manual_seed(K)
     x = torch.randn(K, rows, generator=g).to(dtype).to(gpu)
     check_quantize(x.t())                                    # blocks along the other axis
     wide = torch.randn(K, rows + 13, generator=g).to(dtype).to(gpu)
     check_quantize(wide[:, 5:5 + rows].t())
+    check_quantize(torch.randn(1, rows, generator=g).to(dtype).to(gpu).expand(K, rows).t())
+    bad = x.clone()
+    bad[K // 2, rows // 2], bad[K - 1, 0] = float("nan"), -float("inf")
+    check_quantize(bad.t())
     check_quantize(torch.randn(rows, K + 9, generator=g).to(dtype).to(gpu)[:, 3:3 + K])   # unaligned rows
     check_quantize(torch.randn(rows, 2 * K, generator=g).to(dtype).to(gpu)[:, ::2])
     check_quantize(torch.randn(1, K, generator=g).to(dtype).to(gpu).expand(rows, K))
@@ -502,10 +507,12 @@ def test_c_entries_refuse_bad_sizes():
         L = hk.load()
     except hk.HIPError:
         pytest.skip("the library is not built")
-    assert L.kamd_mxfp4_quantize_launch(0, 0, 0, -1, 32, 32, 0, None) == -1
-    assert L.kamd_mxfp4_quantize_launch(0, 0, 0, 1, 32, 32, 3, None) == -1
-    assert L.kamd_mxfp4_quantize_launch(0, 0, 0, 1, 1 << 40, 32, 0, None) == -1
+    assert L.kamd_mxfp4_quantize_launch(0, 0, 0, -1, 32, 32, 1, 0, None) == -1
+    assert L.kamd_mxfp4_quantize_launch(0, 0, 0, 1, 32, 32, 1, 3, None) == -1
+    assert L.kamd_mxfp4_quantize_launch(0, 0, 0, 1, 1 << 40, 32, 1, 0, None) == -1
     assert b"too large" in L.kamd_hip_last_error()
+    assert L.kamd_mxfp4_quantize_launch(0, 0, 0, 4, 64, 128, 2, 0, None) == -1
+    assert L.kamd_mxfp4_quantize_launch(0, 8, 0, 4, 64, 64, 1, 0, None) == -1
     assert L.kamd_mxfp4_dequantize_launch(0, 0, 0, 1, -1, 0, None) == -1
     assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, -1, 1, 1, 1.0, 1, None, 0, None) == -1
     assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, 1, 1 << 40, 1, 1.0, 1, None, 0, None) == -1
