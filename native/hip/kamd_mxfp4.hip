@@ -32,6 +32,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));   // where values of 2 bytes may lie
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 enum Type { BF16 = 0, FP16 = 1, FP32 = 2 };   // the C entries' type codes
@@ -135,7 +136,10 @@ quantize_rows_kernel(const void* __restrict__ xv, uint32_t* __restrict__ q, uint
   m = max(m, (uint32_t)__shfl_xor((int)m, 1));
   m = max(m, (uint32_t)__shfl_xor((int)m, 2));
   const uint32_t s = scale_byte(m);
-  q[i] = s == 255 ? 0u : o.codes(__uint_as_float(s << 23));
+  const uint32_t c = s == 255 ? 0u : o.codes(__uint_as_float(s << 23));
+  // past the caches: 8192x8192 from fp32 42 against 49 us, but from bf16 31 against 28
+  if constexpr (TYPE == FP32) __builtin_nontemporal_store(c, q + i);
+  else q[i] = c;
   if ((threadIdx.x & 3) == 0) scale[i >> 2] = (uint8_t)s;
 }
 
@@ -143,7 +147,7 @@ quantize_rows_kernel(const void* __restrict__ xv, uint32_t* __restrict__ q, uint
 // reads 32 rows of memory, 256 bytes of each, a lane having all 32 values of COLS blocks; 8 blocks of a row go
 // through LDS, so that whole cache lines are written. Rows of memory and columns behind the last read as 0.
 template <int TYPE>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
 quantize_cols_kernel(const void* __restrict__ xv, uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int64_t M, int64_t K,
                      int64_t ld, int64_t nb) {
   typedef typename Elem<TYPE>::bits bits;
@@ -154,7 +158,8 @@ quantize_cols_kernel(const void* __restrict__ xv, uint8_t* __restrict__ q, uint8
   const int64_t tiles_m = (M + ROWS - 1) / ROWS;
   const int64_t m0 = (int64_t)blockIdx.x % tiles_m * ROWS, b0 = (int64_t)blockIdx.x / tiles_m * 8;
   const int64_t m = m0 + lane * COLS;
-  for (int b = wave * 2; b < wave * 2 + 2; ++b) {
+  {
+    const int b = wave;
     const int64_t k0 = (b0 + b) * 32;
     const bits* p = (const bits*)xv + k0 * ld + m;
     uint32_t v[32];
@@ -208,8 +213,8 @@ quantize_cols_kernel(const void* __restrict__ xv, uint8_t* __restrict__ q, uint8
   __syncthreads();
   const int blocks = (int)(nb - b0 < 8 ? nb - b0 : 8);
 #pragma unroll
-  for (int i = 0; i < ROWS / 32; ++i) {
-    const int row = i * 32 + tid / 8, b = tid % 8;
+  for (int i = 0; i < ROWS / 64; ++i) {
+    const int row = i * 64 + tid / 8, b = tid % 8;
     if (m0 + row >= M || b >= blocks) continue;
     const i32x4 v = *(const i32x4*)(codes + row * PITCH + b * 16);
     *((i32x4*)q + (m0 + row) * nb + b0 + b) = v;
@@ -224,40 +229,48 @@ quantize_cols_kernel(const void* __restrict__ xv, uint8_t* __restrict__ q, uint8
   }
 }
 
-// The inverse, rounded once to the output's type. v_cvt_scalef32_pk_*_fp4 gives NaN for s = 255.
-template <int TYPE>
+// The inverse, rounded once to the output's type: v_cvt_scalef32_pk_*_fp4, which gives NaN for s = 255. A lane makes
+// 16 bytes, 8 values of 16 bits or 4 of 32, so that a wave's store is one run. STREAM: stores that leave the caches
+// alone, for rows of whole 16 bytes (8192x8192 to fp32: 42 against 64 us, 16384x16384 to bf16: 93 and 126, 2048x4096:
+// 3.8 and 4.7); with others they meet cache lines in parts (5000x8001 to fp32: 35 against 31 us).
+template <int TYPE, bool STREAM>
 __global__ void __launch_bounds__(256)
-dequantize_kernel(const uint32_t* __restrict__ q, const uint8_t* __restrict__ scale, void* __restrict__ xv,
-                  size_t first, size_t items, uint32_t row_items, int64_t K) {
+dequantize_kernel(const void* __restrict__ qv, const uint8_t* __restrict__ scale, void* __restrict__ xv, size_t first,
+                  size_t items, uint32_t row_items, int64_t K) {
   typedef typename Elem<TYPE>::bits bits;
+  constexpr int V = 16 / (int)sizeof(bits);
   const size_t base = first + (size_t)blockIdx.x * 256;
   const size_t i = base + threadIdx.x;
   if (i >= items) return;
   const size_t row0 = base / row_items;
   const uint32_t at = (uint32_t)(base - row0 * row_items) + threadIdx.x, over = at / row_items;
-  const int64_t k0 = (int64_t)(at - over * row_items) * 8;
-  const uint32_t c = q[i];
-  const float s = __uint_as_float((uint32_t)scale[i >> 2] << 23);
-  bits t[8];
+  const int64_t k0 = (int64_t)(at - over * row_items) * V;
+  const float s = __uint_as_float((uint32_t)scale[i / (32 / V)] << 23);
+  u32x4_any w;
   if constexpr (TYPE == FP32) {
-    const f32x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1),
-                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3)};
-    __builtin_memcpy(t, v, sizeof t);
+    const uint32_t c = ((const uint16_t*)qv)[i];
+    const f32x2 v[2] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1)};
+    __builtin_memcpy(&w, v, 16);
   } else if constexpr (TYPE == BF16) {
+    const uint32_t c = ((const uint32_t*)qv)[i];
     const bf16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1),
                          __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3)};
-    __builtin_memcpy(t, v, sizeof t);
+    __builtin_memcpy(&w, v, 16);
   } else {
+    const uint32_t c = ((const uint32_t*)qv)[i];
     const f16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 1),
                         __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 3)};
-    __builtin_memcpy(t, v, sizeof t);
+    __builtin_memcpy(&w, v, 16);
   }
   bits* p = (bits*)xv + (int64_t)(row0 + over) * K + k0;
-  if (k0 + 8 <= K) {
-    __builtin_memcpy(p, t, sizeof t);
+  if (k0 + V <= K) {
+    if constexpr (STREAM) __builtin_nontemporal_store(w, (u32x4_any*)p);
+    else *(u32x4_any*)p = w;
   } else {
+    bits t[V];
+    __builtin_memcpy(t, &w, 16);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < V; ++j)
       if (k0 + j < K) p[j] = t[j];
   }
 }
@@ -767,13 +780,12 @@ gemm_rows_kernel(const uint8_t* __restrict__ P, const uint8_t* __restrict__ Ps, 
 constexpr size_t SLICE = (size_t)1 << 31;
 
 template <typename F>
-static int sliced(size_t items, const char* what, F launch) {
+static int sliced(size_t items, F launch) {
   for (size_t first = 0; first < items; first += SLICE) {
     const size_t n = items - first < SLICE ? items - first : SLICE;
     launch(first, dim3((unsigned)((n + 255) / 256)));
     HC(hipGetLastError());
   }
-  (void)what;
   return 0;
 }
 
@@ -912,13 +924,13 @@ int kamd_mxfp4_quantize_launch(const void* x, void* q, void* scale, int64_t rows
   if (((uintptr_t)q) & 15) return kamd_fail("mxfp4_quantize: codes must be 16-byte aligned");
   if (step != 1 && K > 1) {
     const int64_t tile = type == FP32 ? 64 : 128, tiles = (rows + tile - 1) / tile * ((nb + 7) / 8);
-    if (tiles >= (int64_t)1 << 24) return kamd_fail("mxfp4_quantize: %lld x %lld is too large", (long long)rows, (long long)K);
+    if (tiles >= (int64_t)1 << 23) return kamd_fail("mxfp4_quantize: %lld x %lld is too large", (long long)rows, (long long)K);
     auto k = type == BF16 ? quantize_cols_kernel<BF16> : type == FP16 ? quantize_cols_kernel<FP16> : quantize_cols_kernel<FP32>;
-    hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(256), 0, stream, x, (uint8_t*)q, (uint8_t*)scale, rows, K, step, nb);
+    hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(512), 0, stream, x, (uint8_t*)q, (uint8_t*)scale, rows, K, step, nb);
     return kamd_check(hipGetLastError(), "mxfp4_quantize launch");
   }
   const size_t items = (size_t)rows * row_items;
-  return sliced(items, "mxfp4_quantize", [&](size_t first, dim3 grid) {
+  return sliced(items, [&](size_t first, dim3 grid) {
     auto k = type == BF16 ? quantize_rows_kernel<BF16> : type == FP16 ? quantize_rows_kernel<FP16> : quantize_rows_kernel<FP32>;
     hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, x, (uint32_t*)q, (uint8_t*)scale, first, items, (uint32_t)row_items, K,
                        row_step);
@@ -928,17 +940,21 @@ int kamd_mxfp4_quantize_launch(const void* x, void* q, void* scale, int64_t rows
 // the inverse into contiguous rows of K values; q is 4-byte aligned
 int kamd_mxfp4_dequantize_launch(const void* q, const void* scale, void* x, int64_t rows, int64_t K, int type,
                                  hipStream_t stream) {
+  using namespace mxfp4;
   if (rows < 0 || K < 0 || type < 0 || type > 2) return kamd_fail("mxfp4_dequantize: bad arguments");
   if (rows == 0 || K == 0) return 0;
-  const int64_t row_items = (K + 31) / 32 * 4;
+  const int64_t row_items = (K + 31) / 32 * (type == FP32 ? 8 : 4);
   if (row_items >= (int64_t)1 << 31) return kamd_fail("mxfp4_dequantize: K (%lld) is too large", (long long)K);
   const size_t items = (size_t)rows * row_items;
-  return mxfp4::sliced(items, "mxfp4_dequantize", [&](size_t first, dim3 grid) {
-    auto k = type == mxfp4::BF16   ? mxfp4::dequantize_kernel<mxfp4::BF16>
-             : type == mxfp4::FP16 ? mxfp4::dequantize_kernel<mxfp4::FP16>
-                                   : mxfp4::dequantize_kernel<mxfp4::FP32>;
-    hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, (const uint32_t*)q, (const uint8_t*)scale, x, first, items,
-                       (uint32_t)row_items, K);
+  const bool stream_out = K * (type == FP32 ? 4 : 2) % 16 == 0 && ((uintptr_t)x & 15) == 0;
+  return sliced(items, [&](size_t first, dim3 grid) {
+    auto k = stream_out ? (type == BF16   ? dequantize_kernel<BF16, true>
+                           : type == FP16 ? dequantize_kernel<FP16, true>
+                                          : dequantize_kernel<FP32, true>)
+                        : (type == BF16   ? dequantize_kernel<BF16, false>
+                           : type == FP16 ? dequantize_kernel<FP16, false>
+                                          : dequantize_kernel<FP32, false>);
+    hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, q, (const uint8_t*)scale, x, first, items, (uint32_t)row_items, K);
   });
 }
 
