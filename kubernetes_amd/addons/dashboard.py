@@ -47,6 +47,7 @@ async def summary(client: Client) -> dict:
                          "numa": a.get(core.ATTR_NUMA, ""), "partition": a.get(core.ATTR_PARTITION, "SPX"),
                          "socket": a.get(core.ATTR_SOCKET, ""), "burn_in": a.get("amd.com/burn-in", ""),
                          "tflops": a.get("amd.com/mfma-tflops", ""), "fp8_tflops": a.get("amd.com/mfma-fp8-tflops", ""),
+                         "fp4_tflops": a.get("amd.com/mfma-fp4-tflops", ""),
                          "pod": used.get((name, did), "")})
         node_rows.append({"name": name, "ready": ready, "unschedulable": bool((n.get("spec") or {}).get("unschedulable")),
                           "gpus": len(devs), "allocated": sum(1 for r in rows if r["pod"]),
@@ -77,9 +78,10 @@ def render(s: dict) -> str:
             for d in n["devices"]:
                 cls = "" if d["health"] == core.HEALTHY else " class='bad'"
                 part = d["partition"] + (f"@{d['socket']}" if d["partition"] != "SPX" else "")
+                fp4 = f" / fp4 {e(d['fp4_tflops'])}" if d.get("fp4_tflops") else ""
                 out.append(f"<tr><td>{e(d['id'])}</td><td{cls}>{e(str(d['health']))}</td><td>{e(d['hive'])}</td>"
                            f"<td>{e(d['numa'])}</td><td>{e(part)}</td><td>{e(d['burn_in'])}</td>"
-                           f"<td>{e(d['tflops'])} / {e(d['fp8_tflops'])}</td><td>{e(d['pod'])}</td></tr>")
+                           f"<td>{e(d['tflops'])} / {e(d['fp8_tflops'])}{fp4}</td><td>{e(d['pod'])}</td></tr>")
             out.append("</table>")
     out.append("<h2>Pods</h2><table><tr><th>namespace</th><th>name</th><th>phase</th><th>node</th><th>GPUs</th></tr>")
     for p in s["pods"]:

@@ -28,6 +28,8 @@ def main(argv=None):
     ap.add_argument("--burn-in-min-hbm-gbps", type=float, default=3000.0)
     ap.add_argument("--burn-in-min-fp8-tflops", type=float, default=1400.0,
                     help="fp8 (e4m3, block-scaled MFMA) GEMM floor; 0 skips the fp8 step")
+    ap.add_argument("--burn-in-min-fp4-tflops", type=float, default=0.0,
+                    help="microscaled fp4 GEMM floor (half of what a healthy MI355X measures is 2000); 0 skips the fp4 step")
     ap.add_argument("--xgmi-link-probe", action="store_true",
                     help="measure peer copies between the node's GPUs (xgmi-probe --p2p) after burn-in; "
                          "links below --xgmi-link-min-gbps leave the published link graph")
@@ -43,7 +45,8 @@ def main(argv=None):
         if a.burn_in:
             from ..deviceplugin.burnin import BurnIn
             burn_in = BurnIn(min_tflops=a.burn_in_min_tflops, min_hbm_gbps=a.burn_in_min_hbm_gbps,
-                             min_fp8_tflops=a.burn_in_min_fp8_tflops, fp8=a.burn_in_min_fp8_tflops > 0)
+                             min_fp8_tflops=a.burn_in_min_fp8_tflops, fp8=a.burn_in_min_fp8_tflops > 0,
+                             min_fp4_tflops=a.burn_in_min_fp4_tflops)
         probe = None
         if a.xgmi_link_probe and not smi.is_fake:
             from ..deviceplugin.linkprobe import run_probe

@@ -488,7 +488,8 @@ def describe(obj, events=(), ctx=None):
                 if a.get("amd.com/burn-in"):
                     extra += f" burn-in={a['amd.com/burn-in']}"
                     if a.get("amd.com/mfma-tflops"):
-                        extra += (f" (bf16 {a['amd.com/mfma-tflops']} / fp8 {a.get('amd.com/mfma-fp8-tflops', '-')} TF/s,"
+                        fp4 = f" / fp4 {a['amd.com/mfma-fp4-tflops']}" if a.get("amd.com/mfma-fp4-tflops") else ""
+                        extra += (f" (bf16 {a['amd.com/mfma-tflops']} / fp8 {a.get('amd.com/mfma-fp8-tflops', '-')}{fp4} TF/s,"
                                   f" HBM {a.get('amd.com/hbm-gbps', '-')} GB/s)")
                 lines.append(f"  {did}  {d.get('health')}  {a.get(core.ATTR_PRODUCT, '')} {a.get(core.ATTR_ARCH, '')} "
                              f"hbm={a.get(core.ATTR_HBM, '')} hive={a.get(core.ATTR_HIVE, '')} numa={a.get(core.ATTR_NUMA, '')} "

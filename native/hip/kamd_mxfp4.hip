@@ -6,12 +6,12 @@
 // zero codes behind K; scales scale[row][nb] bytes. A row is whole 16-byte chunks, one a block, whatever
 // K is, so no kernel below meets a code that straddles a row.
 #include <hip/hip_runtime.h>
-#include <math.h>
 #include <stdint.h>
 #include <string.h>
 
 #include <atomic>
-#include <new>
+#include <cmath>
+#include <exception>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -395,7 +395,7 @@ constexpr int waitcnt(int vm, int lgkm) { return (vm & 15) | (vm >> 4) << 14 | 7
 template <typename OutT, int TM, int TN, int STAGES, bool ARRANGED>
 __global__ void __launch_bounds__(256, TM == 4 ? 1 : 2)
 gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, const uint8_t* __restrict__ B,
-                 const uint8_t* __restrict__ Bs, OutT* __restrict__ C, int M, int N, int nb, float alpha) {
+                 const uint8_t* __restrict__ Bs, OutT* __restrict__ C, int M, int N, int nb, float alpha, int stream) {
   constexpr int BM = 64 * TM, BN = 64 * TN;
   constexpr int DATA = (BM + BN) * 128;
   constexpr bool ACC = TM * TN == 16;
@@ -639,7 +639,9 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
     for (int k = 0; k < 32 / ROWS; ++k) {
       const int row = k * ROWS + lane / LANES, at = lane % LANES * 16;
       const i32x4 v = *(const i32x4*)(mine + row * PITCH + at);
-      __builtin_memcpy(p + (size_t)row * N * sizeof(OutT) + at, &v, 16);
+      u32x4_any* to = (u32x4_any*)(p + (size_t)row * N * sizeof(OutT) + at);
+      if (stream) __builtin_nontemporal_store(__builtin_bit_cast(u32x4_any, v), to);
+      else *to = __builtin_bit_cast(u32x4_any, v);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -776,6 +778,18 @@ gemm_rows_kernel(const uint8_t* __restrict__ P, const uint8_t* __restrict__ Ps, 
   }
 }
 
+// bf16 values, uniform in [-1, 1), by their index: the burn-in's operands
+__global__ void __launch_bounds__(256) fill_kernel(uint16_t* __restrict__ x, size_t n) {
+  const size_t stride = (size_t)gridDim.x * 256;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+    uint32_t h = (uint32_t)i * 2654435761u ^ (uint32_t)(i >> 32);
+    h ^= h >> 15;
+    h *= 0x2c1b3c6du;
+    h ^= h >> 13;
+    x[i] = __builtin_bit_cast(uint16_t, (__bf16)((float)(h & 0xffffff) / 8388608.f - 1.f));
+  }
+}
+
 // A launch's workgroups times 256 lanes stay below 2^32; longer runs take several launches.
 constexpr size_t SLICE = (size_t)1 << 31;
 
@@ -843,8 +857,12 @@ static int launch_tile(const void* A, const void* As, const void* B, const void*
   }
   static std::atomic<uint64_t> asked{0};
   if (allow_lds(kernel, LDS, asked) != 0) return -1;
+  // C past the caches, where its rows are whole 16 bytes: 2048x1024x4096 10.8 against 11.5 us, 8192x8192x2048 to bf16 94
+  // and 102; not a large one of a short K (8192x8192x1024 to fp32: 92 against 82 us)
+  const size_t row = (size_t)N * sizeof(OutT);
+  const bool past_caches = row % 16 == 0 && ((uintptr_t)C & 15) == 0 && (row * M <= (size_t)160 << 20 || nb >= 128);
   hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), LDS, stream, (const uint8_t*)A, (const uint8_t*)As,
-                     (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, alpha);
+                     (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, alpha, (int)past_caches);
   return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
 }
 
@@ -975,6 +993,104 @@ int kamd_gemm_mxfp4_nt_launch(const void* A, const void* As, const void* B, cons
   if ((((uintptr_t)A) | ((uintptr_t)B)) & 15) return kamd_fail("gemm_mxfp4_nt: A/B must be 16-byte aligned");
   return out_fp32 ? mxfp4::launch_gemm<float>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream)
                   : mxfp4::launch_gemm<__bf16>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);
+}
+
+// fp4 burn-in, the protocol of kamd_diag_mfma: random bf16 operands of size x size are quantised on the device, then
+// `iters` products timed. Sampled rows are checked on the host: their codes and scales against the definition, which
+// they have to meet exactly (else the error is 1), and outputs against a product of the codes in 64 bits, relative
+// to the sum of magnitudes. size is a multiple of 32.
+int kamd_diag_mfma_fp4(int dev, int size, int iters, double* tflops, double* max_rel_err) {
+  using namespace mxfp4;
+  if (size < 32 || size % 32 || iters < 1)
+    return kamd_fail("diag_mfma_fp4: size (%d) must be a multiple of 32, iterations (%d) at least 1", size, iters);
+  HC(hipSetDevice(dev));
+  const size_t n = size, nb = n / 32;
+  uint8_t* mem = nullptr;   // x | codes of A, B | C | scales of A, B | workspace
+  const size_t at_q = n * n * 2 * 2, at_c = at_q + n * n, at_s = at_c + n * n * 4, at_w = (at_s + 2 * n * nb + 255) & ~(size_t)255;
+  const int64_t ws = kamd_gemm_mxfp4_nt_workspace(size, size, (int64_t)nb);
+  HC(hipMalloc(&mem, at_w + ws));
+  uint8_t *qa = mem + at_q, *qb = qa + n * n / 2, *sa = mem + at_s, *sb = sa + n * nb;
+  float* c = (float*)(mem + at_c);
+  uint16_t* x = (uint16_t*)mem;
+  hipEvent_t e0 = nullptr, e1 = nullptr;
+  int rc = -1;
+  try {
+    do {
+      hipLaunchKernelGGL(fill_kernel, dim3(1024), dim3(256), 0, 0, x, 2 * n * n);
+      if (kamd_check(hipGetLastError(), "diag_mfma_fp4 fill") != 0) break;
+      if (kamd_mxfp4_quantize_launch(x, qa, sa, size, size, size, 1, BF16, 0) != 0) break;
+      if (kamd_mxfp4_quantize_launch(x + n * n, qb, sb, size, size, size, 1, BF16, 0) != 0) break;
+      auto product = [&] {
+        return kamd_gemm_mxfp4_nt_launch(qa, sa, qb, sb, c, size, size, (int64_t)nb, 1.f, 1, ws ? mem + at_w : nullptr, ws, 0);
+      };
+      if (product() != 0) break;   // warm-up
+      if (kamd_check(hipEventCreate(&e0), "diag_mfma_fp4 event") != 0 || kamd_check(hipEventCreate(&e1), "diag_mfma_fp4 event") != 0) break;
+      if (kamd_check(hipEventRecord(e0, 0), "diag_mfma_fp4 event") != 0) break;
+      bool ok = true;
+      for (int i = 0; i < iters && ok; ++i) ok = product() == 0;
+      if (!ok) break;
+      if (kamd_check(hipEventRecord(e1, 0), "diag_mfma_fp4 event") != 0) break;
+      if (kamd_check(hipEventSynchronize(e1), "diag_mfma_fp4 sync") != 0) break;
+      float ms = 0.f;
+      if (kamd_check(hipEventElapsedTime(&ms, e0, e1), "diag_mfma_fp4 time") != 0) break;
+      *tflops = 2.0 * size * size * (double)size * iters / (ms * 1e-3) / 1e12;
+
+      double worst = 0;
+      std::vector<uint16_t> hx(n);
+      std::vector<uint8_t> hq(n / 2), hs(nb);
+      std::vector<double> va(n), vb(n);
+      auto fetch = [&](const uint16_t* rx, const uint8_t* rq, const uint8_t* rs, std::vector<double>& v) {
+        if (kamd_check(hipMemcpy(hx.data(), rx, n * 2, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") != 0 ||
+            kamd_check(hipMemcpy(hq.data(), rq, n / 2, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") != 0 ||
+            kamd_check(hipMemcpy(hs.data(), rs, nb, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") != 0)
+          return false;
+        static const double grid[8] = {0, 0.5, 1, 1.5, 2, 3, 4, 6};
+        for (size_t b = 0; b < nb; ++b) {
+          double in[32], top = 0;
+          for (int k = 0; k < 32; ++k) {
+            const uint32_t u = (uint32_t)hx[b * 32 + k] << 16;
+            float f;
+            memcpy(&f, &u, 4);
+            in[k] = f;
+            if (fabs(in[k]) > top) top = fabs(in[k]);
+          }
+          const int s = top == 0 ? 0 : ilogb(top) - 2 + 127;
+          if (s != hs[b]) worst = 1;
+          for (int k = 0; k < 32; ++k) {
+            const double w = fabs(ldexp(in[k], 127 - s));
+            const int want = (w > 0.25) + (w >= 0.75) + (w > 1.25) + (w >= 1.75) + (w > 2.5) + (w >= 3.5) + (w > 5);
+            const int code = (hq[(b * 32 + k) / 2] >> (k % 2 * 4)) & 15;
+            if ((code & 7) != want || (code >= 8) != std::signbit(in[k])) worst = 1;
+            v[b * 32 + k] = ldexp(code & 8 ? -grid[code & 7] : grid[code & 7], hs[b] - 127);
+          }
+        }
+        return true;
+      };
+      for (int t = 0; t < 256 && ok; ++t) {
+        const size_t i = (size_t)t * 7919u % n, j = ((size_t)t * 104729u + 13u) % n;
+        float got = 0;
+        ok = fetch(x + i * n, qa + i * n / 2, sa + i * nb, va) && fetch(x + (n + j) * n, qb + j * n / 2, sb + j * nb, vb) &&
+             kamd_check(hipMemcpy(&got, c + i * n + j, 4, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") == 0;
+        double ref = 0, mag = 0;
+        for (size_t k = 0; k < n; ++k) {
+          ref += va[k] * vb[k];
+          mag += fabs(va[k] * vb[k]);
+        }
+        const double err = fabs(got - ref) / (mag > 1e-30 ? mag : 1.0);
+        if (!(err <= worst)) worst = err;   // a NaN as well
+      }
+      if (!ok) break;
+      *max_rel_err = worst;
+      rc = 0;
+    } while (0);
+  } catch (const std::exception& e) {   // no memory on the host
+    kamd_fail("diag_mfma_fp4: %s", e.what());
+    rc = -1;
+  }
+  if (e0) (void)hipEventDestroy(e0);
+  if (e1) (void)hipEventDestroy(e1);
+  (void)hipFree(mem);
+  return rc;
 }
 
 }  // extern "C"
