@@ -144,13 +144,14 @@ def _mx_types():
 def _mx_launch(t, what, entry, *args):
     """A launch on the current stream of the tensor's device, whichever device is current."""
     import torch
-    index = t.device.index
-    if index == torch.cuda.current_device():
-        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    cuda, index = torch._C, t.device.index   # what torch.cuda.current_device and current_stream ask, 2 us sooner
+    if index == cuda._cuda_getDevice():
+        rc = entry(*args, cuda._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
-    _raise(rc, what)
+            rc = entry(*args, cuda._cuda_getCurrentRawStream(index))
+    if rc:
+        _raise(rc, what)
 
 
 def _mx_pair(q, scale, what):
@@ -199,9 +200,8 @@ def mxfp4_quantize(x):
     _mx_gpu(x, "mxfp4_quantize")
     *lead, K = x.shape
     nb = -(-K // MXFP4_BLOCK)
-    dev, u8 = x.device, torch.uint8
-    q = torch.empty((*lead, 16 * nb), device=dev, dtype=u8)
-    scale = torch.empty((*lead, nb), device=dev, dtype=u8)
+    q = x.new_empty((*lead, 16 * nb), dtype=torch.uint8)
+    scale = x.new_empty((*lead, nb), dtype=torch.uint8)
     if K == 0 or 0 in lead:
         return q, scale
     x2 = x if len(lead) == 1 else x.reshape(-1, K)
@@ -229,8 +229,8 @@ def mxfp4_dequantize(q, scale, k=None, dtype=None):
     if k < 0 or -(-k // MXFP4_BLOCK) != nb:
         raise ValueError(f"mxfp4_dequantize: k={k} does not have {nb} blocks of {MXFP4_BLOCK}")
     _mx_gpu(q, "mxfp4_dequantize")
-    x = torch.empty((*lead, k), device=q.device, dtype=dtype)
-    if x.numel() == 0:
+    x = q.new_empty((*lead, k), dtype=dtype)
+    if k == 0 or 0 in lead:
         return x
     _mx_launch(q, "mxfp4_dequantize", load().kamd_mxfp4_dequantize_launch, q.data_ptr(), scale.data_ptr(), x.data_ptr(),
                scale.numel() // nb, k, code)
@@ -252,9 +252,9 @@ def gemm_mxfp4_nt(a, a_scale, b, b_scale, out_fp32=True, alpha=1.0):
     _mx_gpu(a, "gemm_mxfp4_nt")
     M, N, nb = sa[0], sb[0], sa[1] // 16
     L = load()
-    out = torch.empty((M, N), device=a.device, dtype=torch.float32 if out_fp32 else torch.bfloat16)
+    out = a.new_empty((M, N), dtype=torch.float32 if out_fp32 else torch.bfloat16)
     need = L.kamd_gemm_mxfp4_nt_workspace(M, N, nb) if M > 16 and N > 16 else 0   # none for a few rows
-    ws = torch.empty(need, device=a.device, dtype=torch.uint8) if need else None
+    ws = a.new_empty(need) if need else None
     _mx_launch(a, "gemm_mxfp4_nt", L.kamd_gemm_mxfp4_nt_launch, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
                b_scale.data_ptr(), out.data_ptr(), M, N, nb, float(alpha), 1 if out_fp32 else 0,
                ws.data_ptr() if need else None, need)
