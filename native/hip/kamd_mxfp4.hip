@@ -305,7 +305,7 @@ __device__ __forceinline__ void tile_of(uint32_t w, int tiles_m, int tiles_n, in
 }
 
 // ---------------------------------------------------------------------------
-// Large products. A workgroup of 4 waves makes a BM x BN tile of C, each wave a quarter of TM x TN tiles of
+// Large products. A workgroup of 4 waves makes a tile of C of 64 T x 64 T, each wave a quarter of T x T tiles of
 // 32x32 (v_mfma_scale_f32_32x32x64_f8f6f4: lane l holds chunk l / 32 of row l % 32 and that block's scale).
 // K goes by in tiles of 8 blocks (256 values, 128 B a row), STAGES of them in LDS:
 //   * codes HBM -> LDS without registers (global_load_lds, 16 B a lane), 16-byte slot s of row r holding chunk
@@ -389,18 +389,17 @@ arrange_scales_kernel(const uint8_t* __restrict__ As, const uint8_t* __restrict_
   }
 }
 
-// ARRANGED: As is what arrange_scales_kernel left, of both operands, and Bs is not used.
 constexpr int waitcnt(int vm, int lgkm) { return (vm & 15) | (vm >> 4) << 14 | 7 << 4 | lgkm << 8; }   // s_waitcnt's operand
 
-template <typename OutT, int TM, int TN, int STAGES, bool ARRANGED>
-__global__ void __launch_bounds__(256, TM == 4 ? 1 : 2)
+// ARRANGED: As is what arrange_scales_kernel left, of both operands, and Bs is not used.
+template <typename OutT, int T, int STAGES, bool ARRANGED>
+__global__ void __launch_bounds__(256, T == 4 ? 1 : 2)
 gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, const uint8_t* __restrict__ B,
                  const uint8_t* __restrict__ Bs, OutT* __restrict__ C, int M, int N, int nb, float alpha, int stream) {
-  constexpr int BM = 64 * TM, BN = 64 * TN;
+  constexpr int BM = 64 * T, BN = 64 * T;
   constexpr int DATA = (BM + BN) * 128;
-  constexpr bool ACC = TM * TN == 16;
-  static_assert(TM == TN, "fragments of A and B are read in pairs");
-  static_assert(!ARRANGED || TM == 4, "scales are arranged for panels of 128 rows");
+  constexpr bool ACC = T == 4, DEEP = T == 1;
+  static_assert(!ARRANGED || T == 4, "scales are arranged for panels of 128 rows");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // STAGES x codes of A, B
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, h = lane >> 5;
@@ -429,7 +428,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   // 32 bytes of 4 tiles are read at a time, a batch ahead, lane (r, h) taking tiles 2 h and 2 h + 1; the halves of the
   // wave then swap, each keeping its half of every 8 bytes. Of a short last tile the 8 bytes that end with the row
   // are read, and moved down.
-  constexpr int GROUPS = TM + TN;
+  constexpr int GROUPS = 2 * T;
   struct Scales { uint32_t v[GROUPS]; } sc, sn;   // of A's row groups, then B's: this tile's, the next's
   uint64_t batch[GROUPS][2];
   Scales queue[4];
@@ -440,7 +439,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   } else {
 #pragma unroll
     for (int n = 0; n < GROUPS; ++n)
-      sp[n] = n < TM ? As + (size_t)(m0 + (wm * TM + n) * 32 + r) * nb : Bs + (size_t)(n0 + (wn * TN + n - TM) * 32 + r) * nb;
+      sp[n] = n < T ? As + (size_t)(m0 + (wm * T + n) * 32 + r) * nb : Bs + (size_t)(n0 + (wn * T + n - T) * 32 + r) * nb;
   }
   auto sload = [&](int t) {
     if constexpr (ARRANGED) {
@@ -490,25 +489,27 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
     }
   };
 
-  // Fragments of step s, two at a time, asked for in the first groups of the step before: the last of them is on its
-  // way while the other groups' products run.
-  const int baseA = (wm * 32 * TM + r) * 128, baseB = BM * 128 + (wn * 32 * TN + r) * 128;
-  struct Frags { i32x4 a[TM], b[TN]; } f[2];
+  // Fragments, by step: of a whole tile and the next one, or of a step and the next.
+  const int baseA = (wm * 32 * T + r) * 128, baseB = BM * 128 + (wn * 32 * T + r) * 128;
+  struct Frags { i32x4 a[T], b[T]; } f[DEEP ? 8 : 2];
+  auto read_one = [&](int buffer, auto s, Frags& to, int k) {   // b0 a0 b1 a1 ..
+    const uint8_t* p = lds + buffer * DATA + (((4 * h + s) ^ ((r >> 1) & 7)) << 4);
+    if (k % 2 == 0) to.b[k / 2] = *(const i32x4*)(p + baseB + k / 2 * 4096);
+    else to.a[k / 2] = *(const i32x4*)(p + baseA + k / 2 * 4096);
+  };
+  // Of step s, two at a time, asked for in the first groups of the step before: the last of them is on its way while
+  // the other groups' products run.
   auto read = [&](int buffer, auto s, int pair) {
     if (2 * pair >= GROUPS) return;
-#pragma unroll
-    for (int k = 2 * pair; k < 2 * pair + 2; ++k) {
-      const uint8_t* p = lds + buffer * DATA + (((4 * h + s) ^ ((r >> 1) & 7)) << 4);
-      if (k % 2 == 0) f[s % 2].b[k / 2] = *(const i32x4*)(p + baseB + k / 2 * 4096);
-      else f[s % 2].a[k / 2] = *(const i32x4*)(p + baseA + k / 2 * 4096);
-    }
+    read_one(buffer, s, f[s % 2], 2 * pair);
+    read_one(buffer, s, f[s % 2], 2 * pair + 1);
   };
 
-  f32x16 acc[TM][TN];
+  f32x16 acc[T][T];
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+  for (int i = 0; i < T; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+    for (int j = 0; j < T; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
@@ -516,9 +517,9 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   // the first product, it would be in what that product waits for.
   auto step = [&](auto s, auto ask) {
     unroll<GROUPS>([&](auto k) {
-      unroll<TM * TN>([&](auto p) {
-        if constexpr (p * GROUPS / (TM * TN) == k)
-          mfma32<ACC, s>(acc[p / TN][p % TN], f[s % 2].b[p % TN], f[s % 2].a[p / TN], sc.v[TM + p % TN], sc.v[p / TN]);
+      unroll<T * T>([&](auto p) {
+        if constexpr (p * GROUPS / (T * T) == k)
+          mfma32<ACC, s>(acc[p / T][p % T], f[s % 2].b[p % T], f[s % 2].a[p / T], sc.v[T + p % T], sc.v[p / T]);
       });
       __builtin_amdgcn_sched_barrier(0);
       ask(k);
@@ -552,7 +553,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
     auto clear = [&](auto s) {   // what is behind the last block is multiplied by zeros
       if (!full && !next && 4 * h + s >= rem) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) f[s % 2].a[i] = i32x4{0, 0, 0, 0};
+        for (int i = 0; i < T; ++i) f[s % 2].a[i] = i32x4{0, 0, 0, 0};
       }
     };
     clear(s0);
@@ -584,6 +585,52 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   };
   static_assert(STAGES == 2 || STAGES == 4, "a buffer follows from t % 4");
 
+  // The same for T = 1, whose step has less to multiply than an LDS read takes: it reads the next tile's fragments of
+  // all steps behind the products of its first, and asks for the tile STAGES on behind the second's (2048x1024x4096 to
+  // bf16: 9.3 against 9.8 us, 128x4096x4096: 6.1 and 7.0; for T = 2 it is slower, 12.8 and 11.3).
+  auto deep = [&](int t, auto u, auto full) {
+    constexpr int HERE = u % STAGES, NEXT = (u + 1) % STAGES;
+    Frags* const here = f + (u % 2) * 4;
+    Frags* const ahead = f + ((u + 1) % 2) * 4;
+    const bool next = full || t + 1 < nt;
+    if (full) {
+      landed(std::integral_constant<int, (STAGES - 2) * LOADS>{});
+    } else if (STAGES > 2 && t + 3 < nt) {
+      landed(std::integral_constant<int, STAGES == 4 ? 2 * LOADS : 0>{});
+    } else if (STAGES > 2 && t + 2 < nt) {
+      landed(std::integral_constant<int, STAGES == 4 ? LOADS : 0>{});
+    } else {
+      landed(s0);
+    }
+    unroll<4>([&](auto s) {
+      if (!full && !next && 4 * h + s >= rem) {
+#pragma unroll
+        for (int i = 0; i < T; ++i) here[s].a[i] = i32x4{0, 0, 0, 0};
+      }
+      unroll<T * T>([&](auto p) {
+        mfma32<ACC, s>(acc[p / T][p % T], here[s].b[p % T], here[s].a[p / T], sc.v[T + p % T], sc.v[p / T]);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (s == 0) {
+        if (next)
+          unroll<4>([&](auto v) {
+#pragma unroll
+            for (int k = 0; k < GROUPS; ++k) read_one(NEXT, v, ahead[v], k);
+          });
+      }
+      if constexpr (s == 1) {
+        sask(t, u);
+        if (full || t + STAGES < nt) {
+#pragma unroll
+          for (int j = 0; j < LOADS; ++j) stage(t + STAGES, HERE, j);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    if (next) snext(std::integral_constant<int, (u + 1) % 4>{});
+    return next;
+  };
+
   sload(0);
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) stage(0, 0, j);
@@ -594,36 +641,47 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
 #pragma unroll
   for (int i = 1; i < STAGES; ++i)
 #pragma unroll
-    for (int j = 0; j < (i < STAGES - 1 ? LOADS : LOADS / 2); ++j)
+    for (int j = 0; j < (DEEP || i < STAGES - 1 ? LOADS : LOADS / 2); ++j)
       if (i < nt) stage(i, i, j);
-  if (nt >= STAGES) landed(std::integral_constant<int, (STAGES - 2) * LOADS + LOADS / 2>{});
+  if (nt >= STAGES) landed(std::integral_constant<int, (STAGES - 2) * LOADS + (DEEP ? LOADS : LOADS / 2)>{});
   else landed(s0);
-  unroll<GROUPS>([&](auto k) { read(0, s0, k); });
+  if constexpr (DEEP) {
+    unroll<4>([&](auto v) {
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) read_one(0, v, f[v], k);
+    });
+  } else {
+    unroll<GROUPS>([&](auto k) { read(0, s0, k); });
+  }
+  auto either = [&](int t, auto u, auto full) {
+    if constexpr (DEEP) return deep(t, u, full);
+    else return tile(t, u, full);
+  };
   int t = 0;
   for (; t + 3 + STAGES + INNER < nt; t += 4) {
-    tile(t, s0, yes);
-    tile(t + 1, s1, yes);
-    tile(t + 2, s2, yes);
-    tile(t + 3, s3, yes);
+    either(t, s0, yes);
+    either(t + 1, s1, yes);
+    either(t + 2, s2, yes);
+    either(t + 3, s3, yes);
   }
   for (;;) {
-    if (!tile(t++, s0, no)) break;
-    if (!tile(t++, s1, no)) break;
-    if (!tile(t++, s2, no)) break;
-    if (!tile(t++, s3, no)) break;
+    if (!either(t++, s0, no)) break;
+    if (!either(t++, s1, no)) break;
+    if (!either(t++, s2, no)) break;
+    if (!either(t++, s3, no)) break;
   }
   landed(s0);   // no wave reads codes any more
 
   // Element e of lane (r, h) of a 32x32 tile: column r, row 8 (e / 4) + 4 h + e % 4. 32 rows of C go through the
   // wave's part of LDS at a time, 16 bytes apart from a multiple of the banks.
-  constexpr int ROW = 32 * TN * (int)sizeof(OutT), PITCH = ROW + 16;
+  constexpr int ROW = 32 * T * (int)sizeof(OutT), PITCH = ROW + 16;
   constexpr int LANES = ROW / 16, ROWS = 64 / LANES;   // of a store
   static_assert(32 * PITCH <= tile_lds(BM, BN, STAGES) / 4, "a wave's part of LDS");
   uint8_t* const mine = lds + wave * (tile_lds(BM, BN, STAGES) / 4);
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
+  for (int i = 0; i < T; ++i) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
+    for (int j = 0; j < T; ++j) {
       settle<ACC>(acc[i][j]);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -634,7 +692,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    uint8_t* p = (uint8_t*)(C + (size_t)(m0 + (wm * TM + i) * 32) * N + n0 + wn * 32 * TN);
+    uint8_t* p = (uint8_t*)(C + (size_t)(m0 + (wm * T + i) * 32) * N + n0 + wn * 32 * T);
 #pragma unroll
     for (int k = 0; k < 32 / ROWS; ++k) {
       const int row = k * ROWS + lane / LANES, at = lane % LANES * 16;
@@ -845,7 +903,7 @@ static int launch_tile(const void* A, const void* As, const void* B, const void*
     return kamd_fail("gemm_mxfp4_nt: no tile of %d in %lld x %lld x %lld blocks", BM, (long long)M, (long long)N, (long long)nb);
   const int64_t tiles = ((M + BM - 1) / BM) * ((N + BM - 1) / BM);
   if (tiles >= (int64_t)1 << 24) return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)M, (long long)N);
-  auto kernel = gemm_tile_kernel<OutT, T, T, STAGES, ARRANGED>;
+  auto kernel = gemm_tile_kernel<OutT, T, STAGES, ARRANGED>;
   if (ARRANGED) {
     if (!workspace || workspace_bytes < arranged_bytes(M, N, nb) || ((uintptr_t)workspace & 15))
       return kamd_fail("gemm_mxfp4_nt: needs a workspace of %lld bytes, 16-byte aligned", (long long)arranged_bytes(M, N, nb));
@@ -939,6 +997,7 @@ int kamd_mxfp4_quantize_launch(const void* x, void* q, void* scale, int64_t rows
   if (rows == 0 || K == 0) return 0;
   const int64_t nb = (K + 31) / 32, row_items = nb * 4;
   if (row_items >= (int64_t)1 << 31) return kamd_fail("mxfp4_quantize: K (%lld) is too large", (long long)K);
+  if (!x || !q || !scale) return kamd_fail("mxfp4_quantize: a null pointer");
   if (((uintptr_t)q) & 15) return kamd_fail("mxfp4_quantize: codes must be 16-byte aligned");
   if (step != 1 && K > 1) {
     const int64_t tile = type == FP32 ? 64 : 128, tiles = (rows + tile - 1) / tile * ((nb + 7) / 8);
@@ -963,6 +1022,8 @@ int kamd_mxfp4_dequantize_launch(const void* q, const void* scale, void* x, int6
   if (rows == 0 || K == 0) return 0;
   const int64_t row_items = (K + 31) / 32 * (type == FP32 ? 8 : 4);
   if (row_items >= (int64_t)1 << 31) return kamd_fail("mxfp4_dequantize: K (%lld) is too large", (long long)K);
+  if (!q || !scale || !x) return kamd_fail("mxfp4_dequantize: a null pointer");
+  if (((uintptr_t)q) & 3) return kamd_fail("mxfp4_dequantize: codes must be 4-byte aligned");
   const size_t items = (size_t)rows * row_items;
   const bool stream_out = K * (type == FP32 ? 4 : 2) % 16 == 0 && ((uintptr_t)x & 15) == 0;
   return sliced(items, [&](size_t first, dim3 grid) {
@@ -990,6 +1051,7 @@ int kamd_gemm_mxfp4_nt_launch(const void* A, const void* As, const void* B, cons
   if (M < 0 || N < 0 || nb < 0 || M > most || N > most || nb > most)
     return kamd_fail("gemm_mxfp4_nt: sizes out of range (%lld x %lld x %lld blocks)", (long long)M, (long long)N, (long long)nb);
   if (M == 0 || N == 0) return 0;
+  if (!C || (nb != 0 && (!A || !As || !B || !Bs))) return kamd_fail("gemm_mxfp4_nt: a null pointer");
   if ((((uintptr_t)A) | ((uintptr_t)B)) & 15) return kamd_fail("gemm_mxfp4_nt: A/B must be 16-byte aligned");
   return out_fp32 ? mxfp4::launch_gemm<float>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream)
                   : mxfp4::launch_gemm<__bf16>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);

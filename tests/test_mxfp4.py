@@ -329,6 +329,33 @@ def test_gemm_scale_range_and_nan(gpu, M, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,N,nb", [(3000, 3001, 12), (2600, 2500, 9), (4100, 300, 15)])
+def test_gemm_nan_in_large_tiles(gpu, M, N, nb):
+    """A NaN scale in the first block, in the last of a short tile of K, and in rows that two tiles cover."""
+    a, sa = operand(M, nb, 20)
+    b, sb = operand(N, nb, 21)
+    want = hk.gemm_mxfp4_nt(a, sa, b, sb)
+    for i in (0, 130, M - 200, M - 1):
+        sa[i, nb - 1 if i % 2 else 0] = 255
+        want[i] = float("nan")
+    for j in (7, N - 1):
+        sb[j, nb - 1] = 255
+        want[:, j] = float("nan")
+    torch.testing.assert_close(hk.gemm_mxfp4_nt(a, sa, b, sb), want, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.gpu
+def test_gemm_same_rows_in_any_company(gpu):
+    """A row's outputs are the same values whatever kernel its company has it computed by, where sums are exact."""
+    b, sb = operand(4096, 20, 22)
+    a, sa = operand(4096, 20, 23)
+    want = hk.gemm_mxfp4_nt(a, sa, b, sb)
+    for m in (1, 16, 17, 40, 64, 100, 256, 700, 2048):
+        assert torch.equal(hk.gemm_mxfp4_nt(a[:m], sa[:m], b, sb), want[:m])
+        assert torch.equal(hk.gemm_mxfp4_nt(b, sb, a[:m], sa[:m]).t(), want[:m])
+
+
+@pytest.mark.gpu
 def test_gemm_empty(gpu):
     for M, N, nb in ((0, 4, 2), (4, 0, 2), (0, 0, 0)):
         a, sa = operand(M, nb, 1)
@@ -507,20 +534,30 @@ def test_c_entries_refuse_bad_sizes():
         L = hk.load()
     except hk.HIPError:
         pytest.skip("the library is not built")
-    assert L.kamd_mxfp4_quantize_launch(0, 0, 0, -1, 32, 32, 1, 0, None) == -1
-    assert L.kamd_mxfp4_quantize_launch(0, 0, 0, 1, 32, 32, 1, 3, None) == -1
-    assert L.kamd_mxfp4_quantize_launch(0, 0, 0, 1, 1 << 40, 32, 1, 0, None) == -1
-    assert b"too large" in L.kamd_hip_last_error()
-    assert L.kamd_mxfp4_quantize_launch(0, 0, 0, 4, 64, 128, 2, 0, None) == -1
-    assert L.kamd_mxfp4_quantize_launch(0, 8, 0, 4, 64, 64, 1, 0, None) == -1
-    assert L.kamd_mxfp4_dequantize_launch(0, 0, 0, 1, -1, 0, None) == -1
-    assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, -1, 1, 1, 1.0, 1, None, 0, None) == -1
-    assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, 1, 1 << 40, 1, 1.0, 1, None, 0, None) == -1
-    assert L.kamd_gemm_mxfp4_nt_launch(8, 0, 16, 0, 0, 1, 1, 1, 1.0, 1, None, 0, None) == -1
-    assert b"aligned" in L.kamd_hip_last_error()
-    assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, 0, 1, 1, 1.0, 1, None, 0, None) == 0
+    def refuses(rc, why):
+        assert rc == -1 and why in L.kamd_hip_last_error(), L.kamd_hip_last_error()
+
+    p = 4096    # no pointer: every call is refused before one is used
+    quantize, dequantize, gemm = L.kamd_mxfp4_quantize_launch, L.kamd_mxfp4_dequantize_launch, L.kamd_gemm_mxfp4_nt_launch
+    refuses(quantize(p, p, p, -1, 32, 32, 1, 0, None), b"bad arguments")
+    refuses(quantize(p, p, p, 1, 32, 32, 1, 3, None), b"bad arguments")
+    refuses(quantize(p, p, p, 4, 64, 128, 2, 0, None), b"bad arguments")
+    refuses(quantize(p, p, p, 1, 1 << 40, 32, 1, 0, None), b"too large")
+    refuses(quantize(p, p + 8, p, 4, 64, 64, 1, 0, None), b"aligned")
+    for args in ((None, p, p), (p, None, p), (p, p, None)):
+        refuses(quantize(*args, 4, 64, 64, 1, 0, None), b"null")
+        refuses(dequantize(*args, 4, 64, 0, None), b"null")
+    refuses(dequantize(p, p, p, 1, -1, 0, None), b"bad arguments")
+    refuses(dequantize(p, p, p, 1, 1, -1, None), b"bad arguments")
+    refuses(dequantize(p + 2, p, p, 1, 32, 0, None), b"aligned")
+    refuses(gemm(p, p, p, p, p, -1, 1, 1, 1.0, 1, None, 0, None), b"out of range")
+    refuses(gemm(p, p, p, p, p, 1, 1 << 40, 1, 1.0, 1, None, 0, None), b"out of range")
+    refuses(gemm(p + 8, p, p, p, p, 1, 1, 1, 1.0, 1, None, 0, None), b"aligned")
+    for i in range(5):
+        refuses(gemm(*[None if j == i else p for j in range(5)], 1, 1, 1, 1.0, 1, None, 0, None), b"null")
+    assert gemm(None, None, None, None, None, 0, 1, 1, 1.0, 1, None, 0, None) == 0
     need = L.kamd_gemm_mxfp4_nt_workspace(8192, 8192, 256)
     assert need >= 2 * 8192 * 256 and L.kamd_gemm_mxfp4_nt_workspace(1, 8192, 256) == 0
+    assert L.kamd_gemm_mxfp4_nt_workspace(-5, 8192, 256) == 0 and L.kamd_gemm_mxfp4_nt_workspace(0, 0, 0) == 0
     for ws, size in ((None, need), (16, need - 1), (8, need)):
-        assert L.kamd_gemm_mxfp4_nt_launch(0, 0, 0, 0, 0, 8192, 8192, 256, 1.0, 1, ws, size, None) == -1
-        assert b"workspace" in L.kamd_hip_last_error()
+        refuses(gemm(p, p, p, p, p, 8192, 8192, 256, 1.0, 1, ws, size, None), b"workspace")
