@@ -326,80 +326,20 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int tile_lds(int BM, int BN, int stages) { return stages * (BM + BN) * 128; }
 
-// acc += a b^T with byte S of the scales. ACC: in place in the accumulation registers. The compiler's own form
-// gives the sum another place and moves it back, which with 256 of them costs more than the products. What
-// inline assembly has to see to: 2 wait states after an ordinary instruction's write of an operand (the s_nop),
-// and the wait before a sum is read (settle). Sums are used again 16 instructions later, after any wait there is.
-template <bool ACC, int S>
+template <int S>   // acc += a b^T with byte S of the scales
 __device__ __forceinline__ void mfma32(f32x16& acc, i32x4 a, i32x4 b, uint32_t sa, uint32_t sb) {
-  if constexpr (ACC) {
-    asm volatile(
-        "s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%5,0] op_sel_hi:[%6,%6,0] cbsz:4 blgp:4"
-        : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb), "i"(S & 1), "i"(S >> 1));
-  } else {
-    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(a), frag(b), acc, 4, 4, S, (int)sa, S, (int)sb);
-  }
-}
-template <bool ACC>
-__device__ __forceinline__ void settle(f32x16& acc) {
-  if constexpr (ACC) asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc));
-}
-
-// Scales in the order in which the largest tile's lanes take them: panel (a wave's 128 rows) by tile of K, 64 lanes
-// of 16 bytes, lane (r, h) having 4 blocks of rows r, 32 + r, 64 + r, 96 + r. Read where they lie, a row's 8 bytes a
-// tile cost a cache line each; at 8192^3 that made the product 11 % slower than this kernel and its launch do.
-// A workgroup turns 8 tiles of a panel, 64 bytes a row, over in LDS. Blocks behind the last read as 0, which
-// multiplies zeros.
-__global__ void __launch_bounds__(256)
-arrange_scales_kernel(const uint8_t* __restrict__ As, const uint8_t* __restrict__ Bs, uint8_t* __restrict__ out, int M, int N,
-                      int nb) {
-  constexpr int PITCH = 68;   // 17 banks: 32 rows' words of one tile lie in different ones
-  __shared__ uint8_t rows[128 * PITCH];
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
-  const int nt = (nb + 7) / 8, t0 = (int)blockIdx.y * 8;
-  const int panels_a = (M + 255) / 256 * 2, panel = (int)blockIdx.x;
-  const bool isA = panel < panels_a;
-  const int q = isA ? panel : panel - panels_a, all = isA ? M : N;
-  const int row0 = min(q / 2 * 256, all - 256) + q % 2 * 128;
-  const uint8_t* s = isA ? As : Bs;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = i * 64 + tid / 4, c = t0 * 8 + tid % 4 * 16;
-    const uint8_t* p = s + (size_t)(row0 + row) * nb + c;
-    uint32_t v[4] = {0, 0, 0, 0};
-    if (c + 16 <= nb) {
-      __builtin_memcpy(v, p, 16);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
-        if (c + k < nb) v[k / 4] |= (uint32_t)p[k] << (8 * (k % 4));
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) *(uint32_t*)(rows + row * PITCH + tid % 4 * 16 + k * 4) = v[k];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int t = i * 4 + tid / 64;
-    if (t0 + t >= nt) continue;
-    uint32_t v[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = *(const uint32_t*)(rows + (k * 32 + r) * PITCH + t * 8 + h * 4);
-    __builtin_memcpy(__builtin_assume_aligned(out + (((size_t)panel * nt + t0 + t) * 64 + lane) * 16, 16), v, 16);
-  }
+  acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(a), frag(b), acc, 4, 4, S, (int)sa, S, (int)sb);
 }
 
 constexpr int waitcnt(int vm, int lgkm) { return (vm & 15) | (vm >> 4) << 14 | 7 << 4 | lgkm << 8; }   // s_waitcnt's operand
 
-// ARRANGED: As is what arrange_scales_kernel left, of both operands, and Bs is not used.
-template <typename OutT, int T, int STAGES, bool ARRANGED>
-__global__ void __launch_bounds__(256, T == 4 ? 1 : 2)
+template <typename OutT, int T, int STAGES>
+__global__ void __launch_bounds__(256, 2)
 gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, const uint8_t* __restrict__ B,
                  const uint8_t* __restrict__ Bs, OutT* __restrict__ C, int M, int N, int nb, float alpha, int stream) {
   constexpr int BM = 64 * T, BN = 64 * T;
   constexpr int DATA = (BM + BN) * 128;
-  constexpr bool ACC = T == 4, DEEP = T == 1;
-  static_assert(!ARRANGED || T == 4, "scales are arranged for panels of 128 rows");
+  constexpr bool DEEP = T == 1;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // STAGES x codes of A, B
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, h = lane >> 5;
@@ -417,76 +357,57 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   const uint8_t* const tA = A + (size_t)m0 * row_bytes;
   const uint8_t* const tB = B + (size_t)n0 * row_bytes;
   constexpr int LOADS = (BM + BN) / 32;
-  auto stage = [&](int t, int buffer, int j, bool inner = false) {
+  auto stage = [&](int t, int buffer, int j) {
     uint32_t o = off;
-    if (!inner && t == nt - 1 && chunk >= rem) o -= (uint32_t)(chunk - rem + 1) * 16;   // behind the last block: that one again
+    if (t == nt - 1 && chunk >= rem) o -= (uint32_t)(chunk - rem + 1) * 16;   // behind the last block: that one again
     const uint8_t* p = (j < BM / 32 ? tA + j * 32 * row_bytes : tB + (j - BM / 32) * 32 * row_bytes) + (size_t)t * 128;
     __builtin_amdgcn_global_load_lds((const void*)(p + o), (lds_void*)(lds + buffer * DATA + wave * 1024 + j * 4096), 16, 0, 0);
   };
 
-  // Scales. Arranged, they are a load of 16 bytes a lane for A and one for B, a tile ahead. Where they lie, a row's
-  // 32 bytes of 4 tiles are read at a time, a batch ahead, lane (r, h) taking tiles 2 h and 2 h + 1; the halves of the
-  // wave then swap, each keeping its half of every 8 bytes. Of a short last tile the 8 bytes that end with the row
-  // are read, and moved down.
+  // Scales. A row's 32 bytes of 4 tiles are read at a time, a batch ahead, lane (r, h) taking tiles 2 h and 2 h + 1; the
+  // halves of the wave then swap, each keeping its half of every 8 bytes. Of a short last tile the 8 bytes that end
+  // with the row are read, and moved down.
   constexpr int GROUPS = 2 * T;
-  struct Scales { uint32_t v[GROUPS]; } sc, sn;   // of A's row groups, then B's: this tile's, the next's
+  struct Scales { uint32_t v[GROUPS]; } sc, queue[4];   // of A's row groups, then B's: this tile's, 4 tiles'
   uint64_t batch[GROUPS][2];
-  Scales queue[4];
   const uint8_t* sp[GROUPS];
-  if constexpr (ARRANGED) {
-    sp[0] = As + (size_t)(tm * 2 + wm) * nt * 1024 + lane * 16;
-    sp[1] = As + (size_t)((tiles_m + tn) * 2 + wn) * nt * 1024 + lane * 16;
-  } else {
 #pragma unroll
-    for (int n = 0; n < GROUPS; ++n)
-      sp[n] = n < T ? As + (size_t)(m0 + (wm * T + n) * 32 + r) * nb : Bs + (size_t)(n0 + (wn * T + n - T) * 32 + r) * nb;
-  }
+  for (int n = 0; n < GROUPS; ++n)
+    sp[n] = n < T ? As + (size_t)(m0 + (wm * T + n) * 32 + r) * nb : Bs + (size_t)(n0 + (wn * T + n - T) * 32 + r) * nb;
   auto sload = [&](int t) {
-    if constexpr (ARRANGED) {
-      __builtin_memcpy(&sn.v[0], __builtin_assume_aligned(sp[0] + (size_t)t * 1024, 16), 16);
-      __builtin_memcpy(&sn.v[4], __builtin_assume_aligned(sp[1] + (size_t)t * 1024, 16), 16);
-    } else {
 #pragma unroll
-      for (int n = 0; n < GROUPS; ++n) {
-        const uint8_t* p = sp[n] + (size_t)t * 8 + h * 16;
-        if (t * 8 + 32 <= nb) {
-          __builtin_memcpy(batch[n], p, 16);
-        } else {
+    for (int n = 0; n < GROUPS; ++n) {
+      const uint8_t* p = sp[n] + (size_t)t * 8 + h * 16;
+      if (t * 8 + 32 <= nb) {
+        __builtin_memcpy(batch[n], p, 16);
+      } else {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int at = t + h * 2 + i;
-            if (at >= nt) continue;
-            const int back = at == nt - 1 ? 8 - rem : 0;
-            __builtin_memcpy(&batch[n][i], p + i * 8 - back, 8);
-            batch[n][i] >>= 8 * back;
-          }
+        for (int i = 0; i < 2; ++i) {
+          const int at = t + h * 2 + i;
+          if (at >= nt) continue;
+          const int back = at == nt - 1 ? 8 - rem : 0;
+          __builtin_memcpy(&batch[n][i], p + i * 8 - back, 8);
+          batch[n][i] >>= 8 * back;
         }
       }
     }
   };
-  auto sask = [&](int t, auto u) {   // in tile t, u = t % 4, for what comes behind it
-    if constexpr (ARRANGED) {
-      if (t + 1 < nt) sload(t + 1);
-    } else if constexpr (u == 0) {
+  auto sask = [&](int t, auto u) {   // in tile t, u = t % 4, for the 4 tiles behind these
+    if constexpr (u == 0)
       if (t + 4 < nt) sload(t + 4);
-    }
   };
   auto snext = [&](auto u) {   // to a tile t with u = t % 4
-    if constexpr (ARRANGED) {
-      sc = sn;
-    } else {
-      if constexpr (u == 0) {
+    if constexpr (u == 0) {
 #pragma unroll
-        for (int n = 0; n < GROUPS; ++n)
+      for (int n = 0; n < GROUPS; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap((uint32_t)batch[n][i], (uint32_t)(batch[n][i] >> 32), false, false));
-            queue[i].v[n] = v.x;
-            queue[2 + i].v[n] = v.y;
-          }
-      }
-      sc = queue[u];
+        for (int i = 0; i < 2; ++i) {
+          const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap((uint32_t)batch[n][i], (uint32_t)(batch[n][i] >> 32), false, false));
+          queue[i].v[n] = v.x;
+          queue[2 + i].v[n] = v.y;
+        }
     }
+    sc = queue[u];
   };
 
   // Fragments, by step: of a whole tile and the next one, or of a step and the next.
@@ -519,7 +440,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
     unroll<GROUPS>([&](auto k) {
       unroll<T * T>([&](auto p) {
         if constexpr (p * GROUPS / (T * T) == k)
-          mfma32<ACC, s>(acc[p / T][p % T], f[s % 2].b[p % T], f[s % 2].a[p / T], sc.v[T + p % T], sc.v[p / T]);
+          mfma32<s>(acc[p / T][p % T], f[s % 2].b[p % T], f[s % 2].a[p / T], sc.v[T + p % T], sc.v[p / T]);
       });
       __builtin_amdgcn_sched_barrier(0);
       ask(k);
@@ -545,8 +466,6 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   // Tile t in buffer u % STAGES, u = t % 4. The loads of a tile are spread over the last step of the tile STAGES
   // before it and the first of the next one: they pass the vector memory pipe at 16 cycles each for the whole
   // workgroup. full: all tiles that it asks for are there; else it sees which are, and whether it is the last.
-  // INNER: full ones do not ask for the last either, whose loads take some more instructions (256 tile: 1.5 %).
-  constexpr bool INNER = ARRANGED;
   auto tile = [&](int t, auto u, auto full) {
     constexpr int HERE = u % STAGES, NEXT = (u + 1) % STAGES, BEFORE = (u + STAGES - 1) % STAGES;
     const bool next = full || t + 1 < nt;
@@ -559,7 +478,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
     clear(s0);
     step(s0, [&](auto k) {
       read(HERE, s1, k);
-      if (full || t + STAGES - 1 < nt) stage(t + STAGES - 1, BEFORE, LOADS / 2 + k, full && INNER);
+      if (full || t + STAGES - 1 < nt) stage(t + STAGES - 1, BEFORE, LOADS / 2 + k);
       if constexpr (k == 0) sask(t, u);
     });
     clear(s1);
@@ -578,7 +497,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
     clear(s3);
     step(s3, [&](auto k) {
       if (next) read(NEXT, s0, k);
-      if (full || t + STAGES < nt) stage(t + STAGES, HERE, k, full && INNER);
+      if (full || t + STAGES < nt) stage(t + STAGES, HERE, k);
     });
     if (next) snext(std::integral_constant<int, (u + 1) % 4>{});
     return next;
@@ -608,7 +527,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
         for (int i = 0; i < T; ++i) here[s].a[i] = i32x4{0, 0, 0, 0};
       }
       unroll<T * T>([&](auto p) {
-        mfma32<ACC, s>(acc[p / T][p % T], here[s].b[p % T], here[s].a[p / T], sc.v[T + p % T], sc.v[p / T]);
+        mfma32<s>(acc[p / T][p % T], here[s].b[p % T], here[s].a[p / T], sc.v[T + p % T], sc.v[p / T]);
       });
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (s == 0) {
@@ -658,7 +577,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
     else return tile(t, u, full);
   };
   int t = 0;
-  for (; t + 3 + STAGES + INNER < nt; t += 4) {
+  for (; t + 3 + STAGES < nt; t += 4) {
     either(t, s0, yes);
     either(t + 1, s1, yes);
     either(t + 2, s2, yes);
@@ -682,7 +601,6 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   for (int i = 0; i < T; ++i) {
 #pragma unroll
     for (int j = 0; j < T; ++j) {
-      settle<ACC>(acc[i][j]);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         OutT v[4];
@@ -700,6 +618,245 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
       u32x4_any* to = (u32x4_any*)(p + (size_t)row * N * sizeof(OutT) + at);
       if (stream) __builtin_nontemporal_store(__builtin_bit_cast(u32x4_any, v), to);
       else *to = __builtin_bit_cast(u32x4_any, v);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The largest products: tiles of 256x256 on v_mfma_scale_f32_16x16x128_f8f6f4, a wave having 8x8 of 16x16. The same
+// staging of K, with two steps a tile: step s = 0, 1 gives lane (r, g) = (l % 16, l / 16) the chunk 2 g + s. A CU holds
+// one workgroup, a SIMD one wave, with all 512 registers: 256 of sums, two sets of fragments.
+// At full rate this runs into the card's power, so that what counts is energy: products alone, from registers, of
+// random codes, run at 7.2 PFLOP/s in this form and 6.5 as 32x32x64 (8.3 both, of zeros).
+
+// Scales in the order in which the lanes take them: panel (a wave's 128 rows) by tile of K, 64 lanes of 16 bytes, lane
+// (r, g) having the 16 bits of its chunks 2 g and 2 g + 1 of rows r, 16 + r, .. 112 + r. Read where they lie, a row's 8
+// bytes a tile cost a cache line each; at 8192^3 that made the product 11 % slower than this kernel and its launch do.
+// A workgroup turns 8 tiles of a panel, 64 bytes a row, over in LDS. Blocks behind the last read as 0, which
+// multiplies zeros.
+__global__ void __launch_bounds__(256)
+arrange_scales_kernel(const uint8_t* __restrict__ As, const uint8_t* __restrict__ Bs, uint8_t* __restrict__ out, int M, int N,
+                      int nb) {
+  constexpr int PITCH = 68;   // 17 banks: 16 rows' words of one tile lie in different ones
+  __shared__ uint8_t rows[128 * PITCH];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int nt = (nb + 7) / 8, t0 = (int)blockIdx.y * 8;
+  const int panels_a = (M + 255) / 256 * 2, panel = (int)blockIdx.x;
+  const bool isA = panel < panels_a;
+  const int q = isA ? panel : panel - panels_a, all = isA ? M : N;
+  const int row0 = min(q / 2 * 256, all - 256) + q % 2 * 128;
+  const uint8_t* s = isA ? As : Bs;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = i * 64 + tid / 4, c = t0 * 8 + tid % 4 * 16;
+    const uint8_t* p = s + (size_t)(row0 + row) * nb + c;
+    uint32_t v[4] = {0, 0, 0, 0};
+    if (c + 16 <= nb) {
+      __builtin_memcpy(v, p, 16);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (c + k < nb) v[k / 4] |= (uint32_t)p[k] << (8 * (k % 4));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *(uint32_t*)(rows + row * PITCH + tid % 4 * 16 + k * 4) = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t = i * 4 + tid / 64;
+    if (t0 + t >= nt) continue;
+    uint16_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = *(const uint16_t*)(rows + (k * 16 + r) * PITCH + t * 8 + g * 2);
+    __builtin_memcpy(__builtin_assume_aligned(out + (((size_t)panel * nt + t0 + t) * 64 + lane) * 16, 16), v, 16);
+  }
+}
+
+// acc += a b^T with byte SA, SB of the scales, in place in the accumulation registers. The compiler's own form gives
+// the sum another place and moves it back, which with 256 of them costs more than the products. What inline assembly
+// has to see to: 2 wait states between an ordinary instruction's write of an operand and this one, which the callers
+// keep (with an s_nop before each the kernel is 3 % slower; a test looks for it in the assembly), and the wait before a
+// sum is read, which is settle's. Sums are used again 64 instructions later, after any wait there is.
+template <int SA, int SB>
+__device__ __forceinline__ void mfma16(f32x4& acc, i32x4 a, i32x4 b, uint32_t sa, uint32_t sb) {
+  asm volatile(
+      "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
+      : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb), "i"(SA & 1), "i"(SB & 1), "i"(SA >> 1), "i"(SB >> 1));
+}
+// Once all are waited for, each sum is bound behind that wait.
+__device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+__device__ __forceinline__ void settled(f32x4& acc) { asm volatile("" : "+a"(acc)); }
+
+// S: what arrange_scales_kernel left, of both operands
+template <typename OutT>
+__global__ void __launch_bounds__(256, 1)
+gemm_large_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ B, const uint8_t* __restrict__ S,
+                  OutT* __restrict__ C, int M, int N, int nb, float alpha, int stream) {
+  constexpr int B0 = 256 * 128, DATA = 2 * B0, LOADS = 16;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // 2 x codes of A, B
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int wm = wave >> 1, wn = wave & 1;
+  int tm, tn;
+  const int tiles_m = (M + 255) / 256;
+  tile_of(blockIdx.x, tiles_m, (N + 255) / 256, tm, tn);
+  const int m0 = min(tm * 256, M - 256), n0 = min(tn * 256, N - 256);
+  const int nt = (nb + 7) / 8, rem = nb - (nt - 1) * 8;   // tiles of K, blocks of the last
+
+  // staging: a wave's load takes 8 rows of 128 B, and 32 rows on with the next; inner: not of the last tile
+  const size_t row_bytes = (size_t)nb * 16;
+  const int srow = wave * 8 + (lane >> 3), chunk = (lane & 7) ^ ((srow >> 1) & 7);
+  const uint32_t off = (uint32_t)srow * (uint32_t)row_bytes + chunk * 16;
+  const uint8_t* const tA = A + (size_t)m0 * row_bytes;
+  const uint8_t* const tB = B + (size_t)n0 * row_bytes;
+  auto stage = [&](int t, int buffer, int j, bool inner) {
+    uint32_t o = off;
+    if (!inner && t == nt - 1 && chunk >= rem) o -= (uint32_t)(chunk - rem + 1) * 16;   // behind the last block: that one again
+    const uint8_t* p = (j < 8 ? tA + j * 32 * row_bytes : tB + (j - 8) * 32 * row_bytes) + (size_t)t * 128;
+    __builtin_amdgcn_global_load_lds((const void*)(p + o), (lds_void*)(lds + buffer * DATA + wave * 1024 + j * 4096), 16, 0, 0);
+  };
+
+  // scales of A's 8 row groups and B's, 16 bits each: this tile's and the next's
+  struct Scales { uint32_t a[4], b[4]; } sc, sn;
+  const uint8_t* const sA = S + (size_t)(tm * 2 + wm) * nt * 1024 + lane * 16;
+  const uint8_t* const sB = S + (size_t)((tiles_m + tn) * 2 + wn) * nt * 1024 + lane * 16;
+  auto sload = [&](int t) {
+    __builtin_memcpy(sn.a, __builtin_assume_aligned(sA + (size_t)t * 1024, 16), 16);
+    __builtin_memcpy(sn.b, __builtin_assume_aligned(sB + (size_t)t * 1024, 16), 16);
+  };
+
+  // fragments of a step and the next; 0 .. 7 are B's, 8 .. 15 A's
+  struct Frags { i32x4 b[8], a[8]; } f[2];
+  const int base = r * 128, at[2] = {((2 * g) ^ (r >> 1)) << 4, ((2 * g + 1) ^ (r >> 1)) << 4};
+  auto read = [&](int buffer, auto s, int k) {
+    const uint8_t* p = lds + buffer * DATA + base + at[s];
+    if (k % 2 == 0) f[s].b[k / 2] = *(const i32x4*)(p + B0 + (wn * 8 + k / 2) * 2048);
+    else f[s].a[k / 2] = *(const i32x4*)(p + (wm * 8 + k / 2) * 2048);
+  };
+
+  f32x4 acc[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // Step s on one set: 64 products, and behind product p ask(p) asks for something. Asked for before the first product,
+  // it would be in what that product waits for.
+  auto step = [&](auto s, auto ask) {
+    unroll<64>([&](auto p) {
+      constexpr int i = p / 8, j = p % 8;
+      mfma16<j % 2 * 2 + s, i % 2 * 2 + s>(acc[i][j], f[s].b[j], f[s].a[i], sc.b[j / 2], sc.a[i / 2]);
+      __builtin_amdgcn_sched_barrier(0);
+      ask(p);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  auto landed = [](auto keep) {   // as above
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(waitcnt(keep, 0));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto wait_states = [] {   // between ordinary instructions before and products behind
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 1");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr std::integral_constant<int, 0> s0{};
+  constexpr std::integral_constant<int, 1> s1{};
+  constexpr std::false_type no{};
+  constexpr std::true_type yes{};
+
+  // Tile t in buffer u = t % 2. The loads of a tile are spread over the second step of the tile two before it and the
+  // first of the next: they pass the vector memory pipe at 16 cycles each for the whole workgroup. full: it asks for
+  // no tile that is not there, nor for the last.
+  auto tile = [&](int t, auto u, auto full) {
+    const bool next = full || t + 1 < nt;
+    auto clear = [&](auto s) {   // what is behind the last block is multiplied by zeros
+      if (!full && !next && 2 * g + s >= rem) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[s].a[i] = i32x4{0, 0, 0, 0};
+      }
+      if (!full) wait_states();
+    };
+    clear(s0);
+    step(s0, [&](auto p) {
+      if constexpr (p % 2 == 0 && p / 2 < 16) read(u, s1, p / 2);
+      if constexpr (p % 4 == 1 && p / 4 < 8)
+        if (next) stage(t + 1, 1 - u, LOADS / 2 + p / 4, full);
+      if constexpr (p == 3)
+        if (next) sload(t + 1);
+    });
+    landed(s0);
+    clear(s1);
+    step(s1, [&](auto p) {
+      if constexpr (p % 2 == 0 && p / 2 < 16)
+        if (next) read(1 - u, s0, p / 2);
+      if constexpr (p % 8 == 1 && p / 8 < 8)
+        if (full || t + 2 < nt) stage(t + 2, u, p / 8, full);
+    });
+    if (next) {
+      sc = sn;
+      wait_states();
+    }
+    return next;
+  };
+
+  sload(0);
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) stage(0, 0, j, false);
+  __builtin_amdgcn_s_waitcnt(waitcnt(LOADS, 15));   // the scales have come, outside of any branch, as above
+  sc = sn;
+  if (nt > 1) {
+#pragma unroll
+    for (int j = 0; j < LOADS / 2; ++j) stage(1, 1, j, false);
+    landed(std::integral_constant<int, LOADS / 2>{});
+  } else {
+    landed(s0);
+  }
+#pragma unroll
+  for (int k = 0; k < 16; ++k) read(0, s0, k);
+  int t = 0;
+  for (; t + 4 < nt; t += 2) {
+    tile(t, s0, yes);
+    tile(t + 1, s1, yes);
+  }
+  for (;;) {
+    if (!tile(t++, s0, no)) break;
+    if (!tile(t++, s1, no)) break;
+  }
+  landed(s0);   // no wave reads codes any more
+  settle();
+
+  // element e of lane (r, g) of a 16x16 tile: column r, row 4 g + e. 32 rows of C at a time, as above
+  constexpr int ROW = 128 * (int)sizeof(OutT), PITCH = ROW + 16;
+  constexpr int LANES = ROW / 16, ROWS = 64 / LANES;
+  static_assert(32 * PITCH <= DATA / 2, "a wave's part of LDS");
+  uint8_t* const mine = lds + wave * (DATA / 2);
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        settled(acc[i + h][j]);
+        OutT v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (OutT)(alpha * acc[i + h][j][e]);
+        __builtin_memcpy(__builtin_assume_aligned(mine + (h * 16 + r) * PITCH + (j * 16 + g * 4) * sizeof(OutT), sizeof v), v, sizeof v);
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    uint8_t* p = (uint8_t*)(C + (size_t)(m0 + wm * 128 + i * 16) * N + n0 + wn * 128);
+#pragma unroll
+    for (int k = 0; k < 32 / ROWS; ++k) {
+      const int row = k * ROWS + lane / LANES, to = lane % LANES * 16;
+      const u32x4_any v = __builtin_bit_cast(u32x4_any, *(const i32x4*)(mine + row * PITCH + to));
+      u32x4_any* out = (u32x4_any*)(p + (size_t)row * N * sizeof(OutT) + to);
+      if (stream) __builtin_nontemporal_store(v, out);
+      else *out = v;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -894,33 +1051,48 @@ static int allow_lds(F kernel, int bytes, std::atomic<uint64_t>& asked) {
   return 0;
 }
 
+// C past the caches, where its rows are whole 16 bytes: 2048x1024x4096 10.8 against 11.5 us, 8192x8192x2048 to bf16 94
+// and 102; not a large one of a short K (8192x8192x1024 to fp32: 92 against 82 us).
+static bool past_caches(const void* C, int64_t M, size_t row_bytes, int64_t nb) {
+  return row_bytes % 16 == 0 && ((uintptr_t)C & 15) == 0 && (row_bytes * M <= (size_t)160 << 20 || nb >= 128);
+}
+
 template <typename OutT, int T, int STAGES>
 static int launch_tile(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
-                       int64_t nb, float alpha, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+                       int64_t nb, float alpha, hipStream_t stream) {
   constexpr int BM = 64 * T, LDS = tile_lds(BM, BM, STAGES);
-  constexpr bool ARRANGED = T == 4;
   if (M < BM || N < BM || nb < 8 || nb > 1 << 20)   // what the kernel's addresses assume
     return kamd_fail("gemm_mxfp4_nt: no tile of %d in %lld x %lld x %lld blocks", BM, (long long)M, (long long)N, (long long)nb);
   const int64_t tiles = ((M + BM - 1) / BM) * ((N + BM - 1) / BM);
   if (tiles >= (int64_t)1 << 24) return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)M, (long long)N);
-  auto kernel = gemm_tile_kernel<OutT, T, STAGES, ARRANGED>;
-  if (ARRANGED) {
-    if (!workspace || workspace_bytes < arranged_bytes(M, N, nb) || ((uintptr_t)workspace & 15))
-      return kamd_fail("gemm_mxfp4_nt: needs a workspace of %lld bytes, 16-byte aligned", (long long)arranged_bytes(M, N, nb));
-    const int64_t panels = ((M + 255) / 256 + (N + 255) / 256) * 2;
-    hipLaunchKernelGGL(arrange_scales_kernel, dim3((unsigned)panels, (unsigned)((nb + 63) / 64)), dim3(256), 0, stream,
-                       (const uint8_t*)As, (const uint8_t*)Bs, (uint8_t*)workspace, (int)M, (int)N, (int)nb);
-    HC(hipGetLastError());
-    As = workspace;
-  }
+  auto kernel = gemm_tile_kernel<OutT, T, STAGES>;
   static std::atomic<uint64_t> asked{0};
   if (allow_lds(kernel, LDS, asked) != 0) return -1;
-  // C past the caches, where its rows are whole 16 bytes: 2048x1024x4096 10.8 against 11.5 us, 8192x8192x2048 to bf16 94
-  // and 102; not a large one of a short K (8192x8192x1024 to fp32: 92 against 82 us)
-  const size_t row = (size_t)N * sizeof(OutT);
-  const bool past_caches = row % 16 == 0 && ((uintptr_t)C & 15) == 0 && (row * M <= (size_t)160 << 20 || nb >= 128);
   hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), LDS, stream, (const uint8_t*)A, (const uint8_t*)As,
-                     (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, alpha, (int)past_caches);
+                     (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, alpha,
+                     (int)past_caches(C, M, N * sizeof(OutT), nb));
+  return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
+}
+
+template <typename OutT>
+static int launch_large(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
+                        int64_t nb, float alpha, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  constexpr int LDS = tile_lds(256, 256, 2);
+  if (M < 256 || N < 256 || nb < 8 || nb > 1 << 20)
+    return kamd_fail("gemm_mxfp4_nt: no tile of 256 in %lld x %lld x %lld blocks", (long long)M, (long long)N, (long long)nb);
+  const int64_t tiles_m = (M + 255) / 256, tiles_n = (N + 255) / 256, need = arranged_bytes(M, N, nb);
+  if (tiles_m * tiles_n >= (int64_t)1 << 24) return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)M, (long long)N);
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
+    return kamd_fail("gemm_mxfp4_nt: needs a workspace of %lld bytes, 16-byte aligned", (long long)need);
+  auto kernel = gemm_large_kernel<OutT>;
+  static std::atomic<uint64_t> asked{0};
+  if (allow_lds(kernel, LDS, asked) != 0) return -1;
+  hipLaunchKernelGGL(arrange_scales_kernel, dim3((unsigned)((tiles_m + tiles_n) * 2), (unsigned)((nb + 63) / 64)), dim3(256), 0,
+                     stream, (const uint8_t*)As, (const uint8_t*)Bs, (uint8_t*)workspace, (int)M, (int)N, (int)nb);
+  HC(hipGetLastError());
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * tiles_n)), dim3(256), LDS, stream, (const uint8_t*)A, (const uint8_t*)B,
+                     (const uint8_t*)workspace, (OutT*)C, (int)M, (int)N, (int)nb, alpha,
+                     (int)past_caches(C, M, N * sizeof(OutT), nb));
   return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
 }
 
@@ -971,13 +1143,13 @@ static int launch_gemm(const void* A, const void* As, const void* B, const void*
     return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
   }
   switch (tile_size(M, N, nb)) {
-    case 256: return launch_tile<OutT, 4, 2>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);
+    case 256: return launch_large<OutT>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);
     case 128:
       // one tile a CU: 4 stages; more: 2, and two tiles on a CU (2048x2048x8192: 25 and 30 us, 4096x2048x4096: 32 and 27)
       return ((M + 127) / 128) * ((N + 127) / 128) <= 256
-                 ? launch_tile<OutT, 2, 4>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream)
-                 : launch_tile<OutT, 2, 2>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream);
-    case 64: return launch_tile<OutT, 1, 4>(A, As, B, Bs, C, M, N, nb, alpha, nullptr, 0, stream);
+                 ? launch_tile<OutT, 2, 4>(A, As, B, Bs, C, M, N, nb, alpha, stream)
+                 : launch_tile<OutT, 2, 2>(A, As, B, Bs, C, M, N, nb, alpha, stream);
+    case 64: return launch_tile<OutT, 1, 4>(A, As, B, Bs, C, M, N, nb, alpha, stream);
   }
   // the operand with more rows is P; element (p, q) of the product at p * cp + q * cq
   return M <= N ? launch_rows<OutT>(B, Bs, A, As, C, N, M, nb, 1, N, alpha, stream)
