@@ -692,6 +692,10 @@ __device__ __forceinline__ void mfma16(f32x4& acc, i32x4 a, i32x4 b, uint32_t sa
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 __device__ __forceinline__ void settled(f32x4& acc) { asm volatile("" : "+a"(acc)); }
 
+// Slot s of row r holds chunk s ^ turn(r) here. A quarter of a wave's reads is not 16 lanes in a row: with rows 0 .. 3
+// and 12 .. 15 of one chunk go rows 4 .. 11 of the chunk 2 on, and s ^ (r / 2 % 8) has them meet in half the banks.
+__device__ __forceinline__ int turn(int row) { return ((row >> 1) & 7) ^ (row & 4); }
+
 // S: what arrange_scales_kernel left, of both operands
 template <typename OutT>
 __global__ void __launch_bounds__(256, 1)
@@ -710,7 +714,7 @@ gemm_large_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ B, 
 
   // staging: a wave's load takes 8 rows of 128 B, and 32 rows on with the next; inner: not of the last tile
   const size_t row_bytes = (size_t)nb * 16;
-  const int srow = wave * 8 + (lane >> 3), chunk = (lane & 7) ^ ((srow >> 1) & 7);
+  const int srow = wave * 8 + (lane >> 3), chunk = (lane & 7) ^ turn(srow);
   const uint32_t off = (uint32_t)srow * (uint32_t)row_bytes + chunk * 16;
   const uint8_t* const tA = A + (size_t)m0 * row_bytes;
   const uint8_t* const tB = B + (size_t)n0 * row_bytes;
@@ -732,7 +736,7 @@ gemm_large_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ B, 
 
   // fragments of a step and the next; 0 .. 7 are B's, 8 .. 15 A's
   struct Frags { i32x4 b[8], a[8]; } f[2];
-  const int base = r * 128, at[2] = {((2 * g) ^ (r >> 1)) << 4, ((2 * g + 1) ^ (r >> 1)) << 4};
+  const int base = r * 128, at[2] = {((2 * g) ^ turn(r)) << 4, ((2 * g + 1) ^ turn(r)) << 4};
   auto read = [&](int buffer, auto s, int k) {
     const uint8_t* p = lds + buffer * DATA + base + at[s];
     if (k % 2 == 0) f[s].b[k / 2] = *(const i32x4*)(p + B0 + (wn * 8 + k / 2) * 2048);
@@ -868,8 +872,8 @@ gemm_large_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ B, 
 // with the few; a workgroup makes NP x NQ tiles of 16x16 (v_mfma_scale_f32_16x16x128_f8f6f4), its WAVES taking units
 // of 8 blocks (256 values, 128 B a row) of K in turn, each through two buffers of its own in LDS: no wave waits for
 // another before the sums meet, in the order of the waves. (Straight to registers the instruction's layout has
-// neighbouring lanes read different rows, 16 bytes of each: 32x8192x8192 took 13.3 us so.) Slots in LDS, and what is
-// read behind the last row and block, are as in the tiles above; lane (r, g) takes chunks 2 g and 2 g + 1 of row r,
+// neighbouring lanes read different rows, 16 bytes of each: 32x8192x8192 took 13.3 us so.) Slots in LDS are those of
+// the largest tile, and what is read behind the last row and block is as there; lane (r, g) takes chunks 2 g and 2 g + 1 of row r,
 // whose scales are one 16-bit word, the instruction's byte select taking them apart.
 constexpr int rows_lds(int NP, int NQ, int WAVES) { return WAVES * 2 * (NP + NQ) * 16 * 128; }
 
@@ -890,7 +894,7 @@ gemm_rows_kernel(const uint8_t* __restrict__ P, const uint8_t* __restrict__ Ps, 
   // the block that row i starts with of the 16 GROUPS
   auto row = [&](int i) { return (size_t)(i < NP * 16 ? min(p0 + i, np - 1) : min(q0 + i - NP * 16, nq - 1)) * nb; };
   size_t from[LOADS];   // a load takes 8 rows of 128 B
-  const int chunk[2] = {(lane & 7) ^ (lane >> 4), (lane & 7) ^ (4 + (lane >> 4))};   // of even loads, of odd ones
+  const int chunk[2] = {(lane & 7) ^ turn(lane >> 3), (lane & 7) ^ turn(8 + (lane >> 3))};   // of even loads, of odd ones
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) from[j] = (row(j * 8 + (lane >> 3)) + chunk[j % 2]) * 16;
   size_t srow[GROUPS];
@@ -927,7 +931,7 @@ gemm_rows_kernel(const uint8_t* __restrict__ P, const uint8_t* __restrict__ Ps, 
       i32x4 v[GROUPS];
 #pragma unroll
       for (int i = 0; i < GROUPS; ++i)
-        v[i] = *(const i32x4*)(mine + buffer * UNIT + (i * 16 + r) * 128 + (((2 * g + k) ^ (r >> 1)) << 4));
+        v[i] = *(const i32x4*)(mine + buffer * UNIT + (i * 16 + r) * 128 + (((2 * g + k) ^ turn(r)) << 4));
       if (part && 2 * g + k >= rem) {
 #pragma unroll
         for (int j = 0; j < NQ; ++j) v[NP + j] = i32x4{0, 0, 0, 0};
