@@ -369,7 +369,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
 
   // Scales. A row's 32 bytes of 4 tiles are read at a time, a batch ahead, lane (r, h) taking tiles 2 h and 2 h + 1; the
   // halves of the wave then swap, each keeping its half of every 8 bytes. Of a short last tile the 8 bytes that end
-  // with the row are read, and moved down.
+  // with the row are read, and moved down; where the row has fewer than 8, one by one.
   constexpr int GROUPS = 2 * T;
   struct Scales { uint32_t v[GROUPS]; } sc, queue[4];   // of A's row groups, then B's: this tile's, 4 tiles'
   uint64_t batch[GROUPS][2];
@@ -388,6 +388,11 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
         for (int i = 0; i < 2; ++i) {
           const int at = t + h * 2 + i;
           if (at >= nt) continue;
+          if (nb < 8) {
+            batch[n][i] = 0;
+            for (int k = 0; k < rem; ++k) batch[n][i] |= (uint64_t)p[k] << (8 * k);
+            continue;
+          }
           const int back = at == nt - 1 ? 8 - rem : 0;
           __builtin_memcpy(&batch[n][i], p + i * 8 - back, 8);
           batch[n][i] >>= 8 * back;
@@ -1027,10 +1032,12 @@ static int sliced(size_t items, F launch) {
 // The size of the tiles, in rows and columns: 0 for the small kernel, which takes everything. A round of 256 tiles,
 // one for each CU, takes about 5 and 13 us at K = 4096 for tiles of 64 and 128, and 28 to 42 for 256, whose full rounds
 // run into the power limit (2048x1024: 10.6 against 12.4 us; 2048x2048: 17.5 and 12.7; 4096x2560: 48, 38 and 34;
-// 4096x4096: 74, 51 and 42), in that proportion at any K.
+// 4096x4096: 74, 51 and 42). The proportions hold for other K but for short ones, where all store more than they
+// multiply and 128 and 256 are within a fifth of each other (4096x4096x1024: 21.7 and 23.3 us to fp32;
+// 8192x8192x512: 61 and 65, to bf16 53 and 43).
 static int tile_size(int64_t M, int64_t N, int64_t nb) {
   const int64_t least = M < N ? M : N;
-  if (least < 64 || nb < 8 || nb > 1 << 20) return 0;   // whole tiles inside C, 8 blocks to read, 32-bit offsets in a tile
+  if (least < 64 || nb > 1 << 20) return 0;   // whole tiles inside C, 32-bit offsets in a tile
   auto rounds = [&](int64_t b) { return (((M + b - 1) / b) * ((N + b - 1) / b) + 255) / 256; };
   int best = 64;
   int64_t cost = rounds(64) * 5;
@@ -1067,7 +1074,7 @@ template <typename OutT, int T, int STAGES>
 static int launch_tile(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
                        int64_t nb, float alpha, hipStream_t stream) {
   constexpr int BM = 64 * T, LDS = tile_lds(BM, BM, STAGES);
-  if (M < BM || N < BM || nb < 8 || nb > 1 << 20)   // what the kernel's addresses assume
+  if (M < BM || N < BM || nb < 1 || nb > 1 << 20)   // what the kernel's addresses assume
     return kamd_fail("gemm_mxfp4_nt: no tile of %d in %lld x %lld x %lld blocks", BM, (long long)M, (long long)N, (long long)nb);
   const int64_t tiles = ((M + BM - 1) / BM) * ((N + BM - 1) / BM);
   if (tiles >= (int64_t)1 << 24) return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)M, (long long)N);
@@ -1084,7 +1091,7 @@ template <typename OutT>
 static int launch_large(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
                         int64_t nb, float alpha, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   constexpr int LDS = tile_lds(256, 256, 2);
-  if (M < 256 || N < 256 || nb < 8 || nb > 1 << 20)
+  if (M < 256 || N < 256 || nb < 1 || nb > 1 << 20)
     return kamd_fail("gemm_mxfp4_nt: no tile of 256 in %lld x %lld x %lld blocks", (long long)M, (long long)N, (long long)nb);
   const int64_t tiles_m = (M + 255) / 256, tiles_n = (N + 255) / 256, need = arranged_bytes(M, N, nb);
   if (tiles_m * tiles_n >= (int64_t)1 << 24) return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)M, (long long)N);

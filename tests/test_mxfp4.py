@@ -294,6 +294,19 @@ def test_gemm_large(gpu, M, N, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("nb", [1, 2, 5, 7])
+@pytest.mark.parametrize("M,N", [(64, 64), (97, 130), (2048, 2050), (2304, 1290), (4100, 4111)])
+def test_gemm_short_k(gpu, M, N, nb):
+    """Rows of fewer blocks than a tile has, in tiles of each size."""
+    a, sa = operand(M, nb, 24)
+    b, sb = operand(N, nb, 25)
+    sa[M - 1, nb - 1] = sb[N // 2, 0] = 255
+    want = (values_of(a, sa).to(gpu) @ values_of(b, sb).to(gpu).t()).float()
+    for fp32, dtype in ((True, torch.float32), (False, torch.bfloat16)):
+        torch.testing.assert_close(hk.gemm_mxfp4_nt(a, sa, b, sb, out_fp32=fp32), want.to(dtype), rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M,N,nb", [(1, 33, 40), (40, 70, 9), (128, 300, 32), (300, 520, 40), (512, 512, 64)])
 def test_gemm_wide_scales(gpu, M, N, nb):
     a, sa = operand(M, nb, 5, scales=tuple(range(100, 150)))
@@ -392,7 +405,7 @@ def test_gemm_operands_as_they_come(gpu, M):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("M,N,nb", [(3, 50, 9), (70, 33, 17), (300, 400, 13), (513, 300, 20), (2100, 2050, 9),
-                                    (4100, 4111, 13)])
+                                    (4100, 4111, 13), (70, 65, 3), (2100, 2050, 5), (4100, 4111, 7)])
 def test_gemm_writes_its_output_and_nothing_else(gpu, M, N, nb):
     """Launched into the middle of a larger buffer, the bytes before and behind stay."""
     a, sa = operand(M, nb, 12)
