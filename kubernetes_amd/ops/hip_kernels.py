@@ -253,7 +253,7 @@ def gemm_mxfp4_nt(a, a_scale, b, b_scale, out_fp32=True, alpha=1.0):
     M, N, nb = sa[0], sb[0], sa[1] // 16
     L = load()
     out = a.new_empty((M, N), dtype=torch.float32 if out_fp32 else torch.bfloat16)
-    need = L.kamd_gemm_mxfp4_nt_workspace(M, N, nb) if M > 16 and N > 16 else 0   # none for a few rows
+    need = L.kamd_gemm_mxfp4_nt_workspace(M, N, nb) if nb > 1024 or (M > 16 and N > 16) else 0   # few rows: of a long K only
     ws = a.new_empty(need) if need else None
     _mx_launch(a, "gemm_mxfp4_nt", L.kamd_gemm_mxfp4_nt_launch, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
                b_scale.data_ptr(), out.data_ptr(), M, N, nb, float(alpha), 1 if out_fp32 else 0,

@@ -339,7 +339,7 @@ constexpr int waitcnt(int vm, int lgkm) { return (vm & 15) | (vm >> 4) << 14 | 7
 template <typename OutT, int T, int STAGES>
 __global__ void __launch_bounds__(256, 2)
 gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, const uint8_t* __restrict__ B,
-                 const uint8_t* __restrict__ Bs, OutT* __restrict__ C, int M, int N, int nb, float alpha, int stream) {
+                 const uint8_t* __restrict__ Bs, OutT* __restrict__ C, int M, int N, int nb_all, int per, float alpha, int stream) {
   constexpr int BM = 64 * T, BN = 64 * T;
   constexpr int DATA = (BM + BN) * 128;
   constexpr bool DEEP = T == 1;
@@ -351,14 +351,16 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   const int tiles_m = (M + BM - 1) / BM;
   tile_of(blockIdx.x, tiles_m, (N + BN - 1) / BN, tm, tn);
   const int m0 = min(tm * BM, M - BM), n0 = min(tn * BN, N - BN);
-  const int nt = (nb + 7) / 8, rem = nb - (nt - 1) * 8;   // tiles of K, blocks of the last
+  const int first = (int)blockIdx.y * per;                // this part of K: its blocks, tiles, blocks of the last tile
+  const int nb = min(nb_all - first * 8, per * 8), nt = (nb + 7) / 8, rem = nb - (nt - 1) * 8;
+  C += (size_t)blockIdx.y * M * N;
 
   // staging: a wave's load takes 8 rows of 128 B, and 32 rows on with the next
-  const size_t row_bytes = (size_t)nb * 16;
+  const size_t row_bytes = (size_t)nb_all * 16;
   const int srow = wave * 8 + (lane >> 3), chunk = (lane & 7) ^ ((srow >> 1) & 7);
   const uint32_t off = (uint32_t)srow * (uint32_t)row_bytes + chunk * 16;
-  const uint8_t* const tA = A + (size_t)m0 * row_bytes;
-  const uint8_t* const tB = B + (size_t)n0 * row_bytes;
+  const uint8_t* const tA = A + (size_t)m0 * row_bytes + (size_t)first * 128;
+  const uint8_t* const tB = B + (size_t)n0 * row_bytes + (size_t)first * 128;
   constexpr int LOADS = (BM + BN) / 32;
   auto stage = [&](int t, int buffer, int j) {
     uint32_t o = off;
@@ -376,7 +378,7 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
   const uint8_t* sp[GROUPS];
 #pragma unroll
   for (int n = 0; n < GROUPS; ++n)
-    sp[n] = n < T ? As + (size_t)(m0 + (wm * T + n) * 32 + r) * nb : Bs + (size_t)(n0 + (wn * T + n - T) * 32 + r) * nb;
+    sp[n] = (n < T ? As + (size_t)(m0 + (wm * T + n) * 32 + r) * nb_all : Bs + (size_t)(n0 + (wn * T + n - T) * 32 + r) * nb_all) + first * 8;
   auto sload = [&](int t) {
 #pragma unroll
     for (int n = 0; n < GROUPS; ++n) {
@@ -885,19 +887,21 @@ constexpr int rows_lds(int NP, int NQ, int WAVES) { return WAVES * 2 * (NP + NQ)
 template <typename OutT, int NP, int NQ, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64)
 gemm_rows_kernel(const uint8_t* __restrict__ P, const uint8_t* __restrict__ Ps, const uint8_t* __restrict__ Q,
-                 const uint8_t* __restrict__ Qs, OutT* __restrict__ C, int np, int nq, int nb, int64_t cp, int64_t cq,
-                 float alpha) {
+                 const uint8_t* __restrict__ Qs, OutT* __restrict__ C, int np, int nq, int nb_all, int per, int64_t cp,
+                 int64_t cq, float alpha) {
   constexpr int GROUPS = NP + NQ, UNIT = GROUPS * 16 * 128, LOADS = GROUPS * 2;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int tiles_p = (np + NP * 16 - 1) / (NP * 16);
   const int p0 = (int)(blockIdx.x % tiles_p) * NP * 16, q0 = (int)(blockIdx.x / tiles_p) * NQ * 16;
-  const int units = nb / 8, rem = nb % 8;   // whole units, blocks of a short one
+  const int first = (int)blockIdx.y * per;   // this part of K: its blocks, whole units, blocks of a short one
+  const int nb = min(nb_all - first * 8, per * 8), units = nb / 8, rem = nb % 8;
+  C += (size_t)blockIdx.y * np * nq;
   uint8_t* const mine = lds + wave * 2 * UNIT;
 
   // the block that row i starts with of the 16 GROUPS
-  auto row = [&](int i) { return (size_t)(i < NP * 16 ? min(p0 + i, np - 1) : min(q0 + i - NP * 16, nq - 1)) * nb; };
+  auto row = [&](int i) { return (size_t)(i < NP * 16 ? min(p0 + i, np - 1) : min(q0 + i - NP * 16, nq - 1)) * nb_all + (size_t)first * 8; };
   size_t from[LOADS];   // a load takes 8 rows of 128 B
   const int chunk[2] = {(lane & 7) ^ turn(lane >> 3), (lane & 7) ^ turn(8 + (lane >> 3))};   // of even loads, of odd ones
 #pragma unroll
@@ -1004,6 +1008,17 @@ gemm_rows_kernel(const uint8_t* __restrict__ P, const uint8_t* __restrict__ Ps, 
   }
 }
 
+// The sum of the parts of K, in their order. A part is 4 MiB at most and has just been written: a few microseconds.
+template <typename OutT>
+__global__ void __launch_bounds__(256)
+join_kernel(const float* __restrict__ parts, OutT* __restrict__ C, size_t n, int count, float alpha) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float sum = parts[i];
+  for (int k = 1; k < count; ++k) sum += parts[k * n + i];
+  store_out(C + i, alpha * sum);
+}
+
 // bf16 values, uniform in [-1, 1), by their index: the burn-in's operands
 __global__ void __launch_bounds__(256) fill_kernel(uint16_t* __restrict__ x, size_t n) {
   const size_t stride = (size_t)gridDim.x * 256;
@@ -1047,6 +1062,25 @@ static int tile_size(int64_t M, int64_t N, int64_t nb) {
   return best;
 }
 
+// K in parts, each to workgroups of its own, where a long K falls to half the CUs or fewer; join_kernel adds the sums.
+// A workgroup takes about 0.22 us for a tile of K where its tiles pass through it one by one or its waves are four, and
+// 0.07 with eight waves; the second launch costs 4 us, and the host 5. From 64 and 256 tiles on, in parts of 16 and 32
+// or more: 64x64x16384 14.2 -> 8.3 us, 512x512x65536 83 -> 29, 1x512x65536 23 -> 9; half as long, and nothing is left
+// of the gain (64x64x8192 8.5 and 7.7 us, 1x512x32768 9.5 and 7.7).
+struct Split { int count, per; };   // parts, tiles of K in each
+static Split split_k(int64_t M, int64_t N, int64_t nb) {
+  const int64_t nt = (nb + 7) / 8, tile = tile_size(M, N, nb);
+  const int64_t most = M < N ? N : M, each = ((M < N ? M : N) + 15) / 16;
+  const int64_t groups = tile == 64  ? ((M + 63) / 64) * ((N + 63) / 64)
+                         : tile == 0 ? (most + 15) / 16 * (each <= 2 ? 1 : (each + 3) / 4)
+                                     : 256;
+  const bool eight = tile == 0 && each <= 2;   // as launch_rows takes them
+  if (groups > 128 || nt < (eight ? 256 : 64)) return {1, (int)nt};
+  const int64_t least = eight ? 32 : 16, count = 256 / groups < nt / least ? 256 / groups : nt / least;
+  const int64_t per = (nt + count - 1) / count;
+  return {(int)((nt + per - 1) / per), (int)per};
+}
+
 static int64_t arranged_bytes(int64_t M, int64_t N, int64_t nb) {
   return ((M + 255) / 256 + (N + 255) / 256) * 2 * ((nb + 7) / 8) * 1024;
 }
@@ -1072,7 +1106,7 @@ static bool past_caches(const void* C, int64_t M, size_t row_bytes, int64_t nb) 
 
 template <typename OutT, int T, int STAGES>
 static int launch_tile(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
-                       int64_t nb, float alpha, hipStream_t stream) {
+                       int64_t nb, float alpha, Split split, hipStream_t stream) {
   constexpr int BM = 64 * T, LDS = tile_lds(BM, BM, STAGES);
   if (M < BM || N < BM || nb < 1 || nb > 1 << 20)   // what the kernel's addresses assume
     return kamd_fail("gemm_mxfp4_nt: no tile of %d in %lld x %lld x %lld blocks", BM, (long long)M, (long long)N, (long long)nb);
@@ -1081,9 +1115,9 @@ static int launch_tile(const void* A, const void* As, const void* B, const void*
   auto kernel = gemm_tile_kernel<OutT, T, STAGES>;
   static std::atomic<uint64_t> asked{0};
   if (allow_lds(kernel, LDS, asked) != 0) return -1;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), LDS, stream, (const uint8_t*)A, (const uint8_t*)As,
-                     (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, alpha,
-                     (int)past_caches(C, M, N * sizeof(OutT), nb));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, split.count), dim3(256), LDS, stream, (const uint8_t*)A, (const uint8_t*)As,
+                     (const uint8_t*)B, (const uint8_t*)Bs, (OutT*)C, (int)M, (int)N, (int)nb, split.per, alpha,
+                     (int)(split.count == 1 && past_caches(C, M, N * sizeof(OutT), nb)));
   return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
 }
 
@@ -1111,21 +1145,22 @@ static int launch_large(const void* A, const void* As, const void* B, const void
 
 template <typename OutT, int NP, int NQ, int WAVES>
 static int launch_rows_of(const void* P, const void* Ps, const void* Q, const void* Qs, void* C, int64_t np, int64_t nq,
-                          int64_t nb, int64_t cp, int64_t cq, float alpha, hipStream_t stream) {
+                          int64_t nb, int64_t cp, int64_t cq, float alpha, Split split, hipStream_t stream) {
   constexpr int LDS = rows_lds(NP, NQ, WAVES);
   const int64_t tiles = ((np + NP * 16 - 1) / (NP * 16)) * ((nq + NQ * 16 - 1) / (NQ * 16));
   if (tiles * (WAVES * 64) >= (int64_t)1 << 32) return kamd_fail("gemm_mxfp4_nt: %lld x %lld is too large", (long long)np, (long long)nq);
   auto kernel = gemm_rows_kernel<OutT, NP, NQ, WAVES>;
   static std::atomic<uint64_t> asked{0};
   if (allow_lds(kernel, LDS, asked) != 0) return -1;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(WAVES * 64), LDS, stream, (const uint8_t*)P, (const uint8_t*)Ps,
-                     (const uint8_t*)Q, (const uint8_t*)Qs, (OutT*)C, (int)np, (int)nq, (int)nb, cp, cq, alpha);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, split.count), dim3(WAVES * 64), LDS, stream, (const uint8_t*)P,
+                     (const uint8_t*)Ps, (const uint8_t*)Q, (const uint8_t*)Qs, (OutT*)C, (int)np, (int)nq, (int)nb, split.per,
+                     cp, cq, alpha);
   return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
 }
 
 template <typename OutT>
 static int launch_rows(const void* P, const void* Ps, const void* Q, const void* Qs, void* C, int64_t np, int64_t nq, int64_t nb,
-                       int64_t cp, int64_t cq, float alpha, hipStream_t stream) {
+                       int64_t cp, int64_t cq, float alpha, Split split, hipStream_t stream) {
   // Two tiles of P where one would make more than a workgroup for each CU: half the reads of Q, and one round
   // (16x5000x4096: 4.7 against 5.0 us, 32x5000x4096: 5.8 and 7.9). Eight waves where the workgroups are one for each
   // CU, whose LDS they fill; of more, with four, two lie on a CU (32x8192x8192: 8.9 against 10.0 us with four;
@@ -1133,7 +1168,7 @@ static int launch_rows(const void* P, const void* Ps, const void* Q, const void*
   const int64_t cus = 256, each = (nq + 15) / 16;
   const bool wide = np > 16 * cus;
   const bool many = (np + (wide ? 31 : 15)) / (wide ? 32 : 16) * (each <= 2 ? 1 : (each + 3) / 4) > cus;
-#define KAMD_ROWS(NP, NQ, W) launch_rows_of<OutT, NP, NQ, W>(P, Ps, Q, Qs, C, np, nq, nb, cp, cq, alpha, stream)
+#define KAMD_ROWS(NP, NQ, W) launch_rows_of<OutT, NP, NQ, W>(P, Ps, Q, Qs, C, np, nq, nb, cp, cq, alpha, split, stream)
   if (each == 1) {
     if (wide) return many ? KAMD_ROWS(2, 1, 4) : KAMD_ROWS(2, 1, 8);
     return KAMD_ROWS(1, 1, 8);
@@ -1147,26 +1182,39 @@ static int launch_rows(const void* P, const void* Ps, const void* Q, const void*
 }
 
 template <typename OutT>
+static int launch_small(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N, int64_t nb,
+                        float alpha, bool tiles, Split split, hipStream_t stream) {
+  if (tiles) return launch_tile<OutT, 1, 4>(A, As, B, Bs, C, M, N, nb, alpha, split, stream);
+  // the operand with more rows is P; element (p, q) of the product at p * cp + q * cq
+  return M <= N ? launch_rows<OutT>(B, Bs, A, As, C, N, M, nb, 1, N, alpha, split, stream)
+                : launch_rows<OutT>(A, As, B, Bs, C, M, N, nb, N, 1, alpha, split, stream);
+}
+
+template <typename OutT>
 static int launch_gemm(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N, int64_t nb,
                        float alpha, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  const size_t n = (size_t)M * N;
   if (nb == 0) {
-    const size_t n = (size_t)M * N;
     if (n > SLICE) return kamd_fail("gemm_mxfp4_nt: an empty K with more than 2^31 outputs");
     hipLaunchKernelGGL(zero_kernel<OutT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, (OutT*)C, n);
     return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
   }
-  switch (tile_size(M, N, nb)) {
-    case 256: return launch_large<OutT>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);
-    case 128:
-      // one tile a CU: 4 stages; more: 2, and two tiles on a CU (2048x2048x8192: 25 and 30 us, 4096x2048x4096: 32 and 27)
-      return ((M + 127) / 128) * ((N + 127) / 128) <= 256
-                 ? launch_tile<OutT, 2, 4>(A, As, B, Bs, C, M, N, nb, alpha, stream)
-                 : launch_tile<OutT, 2, 2>(A, As, B, Bs, C, M, N, nb, alpha, stream);
-    case 64: return launch_tile<OutT, 1, 4>(A, As, B, Bs, C, M, N, nb, alpha, stream);
-  }
-  // the operand with more rows is P; element (p, q) of the product at p * cp + q * cq
-  return M <= N ? launch_rows<OutT>(B, Bs, A, As, C, N, M, nb, 1, N, alpha, stream)
-                : launch_rows<OutT>(A, As, B, Bs, C, M, N, nb, N, 1, alpha, stream);
+  const int tile = tile_size(M, N, nb);
+  if (tile == 256) return launch_large<OutT>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);
+  const Split split = split_k(M, N, nb);
+  if (tile == 128)
+    // one tile a CU: 4 stages; more: 2, and two tiles on a CU (2048x2048x8192: 25 and 30 us, 4096x2048x4096: 32 and 27)
+    return ((M + 127) / 128) * ((N + 127) / 128) <= 256
+               ? launch_tile<OutT, 2, 4>(A, As, B, Bs, C, M, N, nb, alpha, split, stream)
+               : launch_tile<OutT, 2, 2>(A, As, B, Bs, C, M, N, nb, alpha, split, stream);
+  if (split.count == 1) return launch_small<OutT>(A, As, B, Bs, C, M, N, nb, alpha, tile == 64, split, stream);
+  const int64_t need = (int64_t)n * 4 * split.count;
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
+    return kamd_fail("gemm_mxfp4_nt: needs a workspace of %lld bytes, 16-byte aligned", (long long)need);
+  if (launch_small<float>(A, As, B, Bs, workspace, M, N, nb, 1.f, tile == 64, split, stream) != 0) return -1;
+  hipLaunchKernelGGL(join_kernel<OutT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, (const float*)workspace, (OutT*)C, n,
+                     split.count, alpha);
+  return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
 }
 }  // namespace mxfp4
 
@@ -1224,7 +1272,10 @@ int kamd_mxfp4_dequantize_launch(const void* q, const void* scale, void* x, int6
 
 // bytes of scratch memory that the product of these sizes needs, 0 for most
 int64_t kamd_gemm_mxfp4_nt_workspace(int64_t M, int64_t N, int64_t nb) {
-  return M > 0 && N > 0 && nb > 0 && mxfp4::tile_size(M, N, nb) == 256 ? mxfp4::arranged_bytes(M, N, nb) : 0;
+  if (M <= 0 || N <= 0 || nb <= 0) return 0;
+  if (mxfp4::tile_size(M, N, nb) == 256) return mxfp4::arranged_bytes(M, N, nb);
+  const int parts = mxfp4::split_k(M, N, nb).count;
+  return parts > 1 ? (int64_t)parts * M * N * 4 : 0;
 }
 
 // C[M, N] = alpha * A B^T, A [M, 16 nb] / As [M, nb], B [N, 16 nb] / Bs [N, nb] contiguous, A and B 16-byte aligned;

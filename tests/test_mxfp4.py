@@ -357,6 +357,56 @@ def test_gemm_nan_in_large_tiles(gpu, M, N, nb):
     torch.testing.assert_close(hk.gemm_mxfp4_nt(a, sa, b, sb), want, rtol=0, atol=0, equal_nan=True)
 
 
+LONG = [(1, 1, 2048), (1, 500, 2041), (16, 100, 2059), (32, 64, 4100), (100, 7, 2304), (40, 70, 515), (300, 48, 519), (64, 64, 505),
+        (64, 64, 1025), (100, 200, 777), (512, 500, 1024)]
+
+
+def long_operand(rows, nb, seed):
+    """Values up to 1.5: sums of some hundred thousand products in steps of 1/4 stay exact in 32 bits."""
+    q, s = operand(rows, nb, seed, scales=(127,))
+    return q & 0xBB, s
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,nb", LONG)
+def test_gemm_long_k(gpu, M, N, nb):
+    """A K that few workgroups would have for themselves is taken in parts. NaN of one part stays."""
+    assert hk.load().kamd_gemm_mxfp4_nt_workspace(M, N, nb) >= 2 * M * N * 4
+    a, sa = long_operand(M, nb, 26)
+    b, sb = long_operand(N, nb, 27)
+    want = (values_of(a, sa).to(gpu) @ values_of(b, sb).to(gpu).t()).float()
+    for _ in range(2):
+        assert torch.equal(hk.gemm_mxfp4_nt(a, sa, b, sb), want)
+    assert torch.equal(hk.gemm_mxfp4_nt(a, sa, b, sb, out_fp32=False), want.to(torch.bfloat16))
+    assert torch.equal(hk.gemm_mxfp4_nt(a, sa, b, sb, alpha=-0.25), -0.25 * want)
+    sa[M - 1, nb - 1] = sb[0, 3] = 255
+    want[M - 1] = want[:, 0] = float("nan")
+    torch.testing.assert_close(hk.gemm_mxfp4_nt(a, sa, b, sb), want, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.gpu
+def test_gemm_long_k_twice_at_once(gpu):
+    """Two products in parts on two streams, and in a graph that is replayed beside them: each has its own sums."""
+    a, sa = long_operand(100, 777, 28)
+    b, sb = long_operand(200, 777, 29)
+    c, sc = long_operand(60, 777, 30)
+    first, second = hk.gemm_mxfp4_nt(a, sa, b, sb), hk.gemm_mxfp4_nt(c, sc, b, sb)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = hk.gemm_mxfp4_nt(a, sa, b, sb)
+    other = torch.cuda.Stream()
+    for _ in range(3):
+        held.zero_()
+        graph.replay()
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            y = [hk.gemm_mxfp4_nt(c, sc, b, sb) for _ in range(5)]
+        x = [hk.gemm_mxfp4_nt(a, sa, b, sb) for _ in range(5)]
+        torch.cuda.synchronize()
+        assert torch.equal(held, first) and all(torch.equal(v, first) for v in x) and all(torch.equal(v, second) for v in y)
+
+
 @pytest.mark.gpu
 def test_gemm_same_rows_in_any_company(gpu):
     """A row's outputs are the same values whatever kernel its company has it computed by, where sums are exact."""
@@ -569,6 +619,8 @@ def test_c_entries_refuse_bad_sizes():
     for i in range(5):
         refuses(gemm(*[None if j == i else p for j in range(5)], 1, 1, 1, 1.0, 1, None, 0, None), b"null")
     assert gemm(None, None, None, None, None, 0, 1, 1, 1.0, 1, None, 0, None) == 0
+    refuses(gemm(p, p, p, p, p, 64, 64, 1024, 1.0, 1, None, 0, None), b"workspace")
+    refuses(gemm(p, p, p, p, p, 1, 64, 4096, 1.0, 1, p, 64 * 4, None), b"workspace")
     need = L.kamd_gemm_mxfp4_nt_workspace(8192, 8192, 256)
     assert need >= 2 * 8192 * 256 and L.kamd_gemm_mxfp4_nt_workspace(1, 8192, 256) == 0
     assert L.kamd_gemm_mxfp4_nt_workspace(-5, 8192, 256) == 0 and L.kamd_gemm_mxfp4_nt_workspace(0, 0, 0) == 0
