@@ -638,7 +638,9 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
 // staging of K, with two steps a tile: step s = 0, 1 gives lane (r, g) = (l % 16, l / 16) the chunk 2 g + s. A CU holds
 // one workgroup, a SIMD one wave, with all 512 registers: 256 of sums, two sets of fragments.
 // At full rate this runs into the card's power, so that what counts is energy: products alone, from registers, of
-// random codes, run at 7.2 PFLOP/s in this form and 6.5 as 32x32x64 (8.3 both, of zeros).
+// random codes, run at 7.2 PFLOP/s in this form and 6.5 as 32x32x64 (8.3 both, of zeros). 8192^3 takes 252 us to fp32
+// and 232 to bf16 with the scales' launch, 4.4 and 4.7 PFLOP/s, at 1.85 of 2.4 GHz, products in 62 % of the cycles; the
+// rest is the write of C at the end of each of 4 rounds, by all CUs at one time (11 us a round to fp32).
 
 // Scales in the order in which the lanes take them: panel (a wave's 128 rows) by tile of K, 64 lanes of 16 bytes, lane
 // (r, g) having the 16 bits of its chunks 2 g and 2 g + 1 of rows r, 16 + r, .. 112 + r. Read where they lie, a row's 8
