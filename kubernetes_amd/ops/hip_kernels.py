@@ -205,6 +205,8 @@ def mxfp4_quantize(x):
     if K == 0 or 0 in lead:
         return q, scale
     x2 = x if len(lead) == 1 else x.reshape(-1, K)
+    if x2.is_neg():   # a view whose values are the negated ones of memory
+        x2 = x2.resolve_neg()
     row_step, step = x2.stride()
     if K > 1 and step != 1 and row_step != 1:   # neither rows nor columns in one piece each
         x2 = x2.contiguous()

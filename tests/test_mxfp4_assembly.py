@@ -103,22 +103,22 @@ def _load(text, symbol):
 CLEAN = """
 f:
 f_begin:
-	v_mov_b32_e32 v1, v2
-	s_nop 1
-	v_mfma_x a[0:3], v[0:3], v[4:7], a[0:3], v8, v9
-	s_nop 15
-	s_nop 1
-	v_accvgpr_read_b32 v10, a0
+    v_mov_b32_e32 v1, v2
+    s_nop 1
+    v_mfma_x a[0:3], v[0:3], v[4:7], a[0:3], v8, v9
+    s_nop 15
+    s_nop 1
+    v_accvgpr_read_b32 v10, a0
 .Lfunc_end0:
 """
 
 
 def test_the_check_finds_what_it_looks_for():
     assert hazards(_load(CLEAN, "f:")) == []
-    assert hazards(_load(CLEAN.replace("s_nop 1\n\tv_mfma", "s_nop 0\n\tv_mfma"), "f:"))
+    assert hazards(_load(CLEAN.replace("s_nop 1\n    v_mfma", "s_nop 0\n    v_mfma"), "f:"))
     assert hazards(_load(CLEAN.replace("s_nop 15\n", "s_nop 8\n"), "f:"))
-    loop = CLEAN.replace("\tv_mov_b32_e32 v1, v2\n\ts_nop 1\n", "\ts_nop 1\n.LBB0_1:\n").replace(
-        "\ts_nop 15\n", "\tv_mov_b32_e32 v9, v2\n\ts_cbranch_scc1 .LBB0_1\n\ts_nop 15\n")
+    loop = CLEAN.replace("    v_mov_b32_e32 v1, v2\n    s_nop 1\n", "    s_nop 1\n.LBB0_1:\n").replace(
+        "    s_nop 15\n", "    v_mov_b32_e32 v9, v2\n    s_cbranch_scc1 .LBB0_1\n    s_nop 15\n")
     assert hazards(_load(loop, "f:"))          # over the back edge: one wait state, the branch
     assert hazards(_load(loop.replace("v_mov_b32_e32 v9", "v_mov_b32_e32 v20"), "f:")) == []
 
