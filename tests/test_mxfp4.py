@@ -212,8 +212,9 @@ def test_quantize_strides(gpu, dtype, rows, K):
 def test_quantize_overlapping_and_negated_views(gpu):
     g = torch.Generator().manual_seed(31)
     row = torch.randn(4 * 96, generator=g).to(gpu)
-    for x in (row[:96].expand(7, 96), row[:70, None].expand(70, 40), row.unfold(0, 96, 1), row.unfold(0, 96, 5),
-              torch.view_as_complex(row.view(4, 48, 2)).conj().imag, torch.view_as_complex(row.view(4, 48, 2)).conj().imag.t(), torch.view_as_complex(row.view(4, 48, 2)).conj().imag[:, 5:6]):
+    imag = torch.view_as_complex(row.view(4, 48, 2)).conj().imag
+    for x in (row[:96].expand(7, 96), row[:70, None].expand(70, 40), row.unfold(0, 96, 1), row.unfold(0, 96, 5), imag,
+              imag.t(), imag[:, 5:6]):
         check_quantize(x)
 
 
