@@ -141,10 +141,10 @@ def _mx_types():
     return _mx_type_codes
 
 
-def _mx_launch(t, what, entry, *args):
-    """A launch on the current stream of the tensor's device, whichever device is current."""
+def _mx_launch(index, what, entry, *args):
+    """A launch on the current stream of that device, whichever device is current."""
     import torch
-    cuda, index = torch._C, t.device.index   # what torch.cuda.current_device and current_stream ask, 2 us sooner
+    cuda = torch._C   # what torch.cuda.current_device and current_stream ask, 2 us sooner
     if index == cuda._cuda_getDevice():
         rc = entry(*args, cuda._cuda_getCurrentRawStream(index))
     else:
@@ -160,7 +160,8 @@ def _mx_pair(q, scale, what):
     u8 = torch.uint8
     qs, ss = q.shape, scale.shape
     if (len(qs) == 2 == len(ss) and q.dtype is u8 is scale.dtype and qs[0] == ss[0] and qs[1] == 16 * ss[1]
-            and q.is_contiguous() and scale.is_contiguous() and q.device == scale.device and not q.data_ptr() % 16):
+            and q.is_contiguous() and scale.is_contiguous() and q.get_device() == scale.get_device() >= 0
+            and not q.data_ptr() % 16):
         return q, scale
     if q.dtype not in (u8, torch.float4_e2m1fn_x2):
         raise ValueError(f"{what}: codes must be uint8 or float4_e2m1fn_x2, got {q.dtype}")
@@ -179,8 +180,11 @@ def _mx_pair(q, scale, what):
 
 
 def _mx_gpu(t, what):
-    if not t.is_cuda:
+    """The index of the tensor's GPU."""
+    index = t.get_device()
+    if index < 0 or not t.is_cuda:
         raise ValueError(f"{what} needs tensors on the GPU, got {t.device}")
+    return index
 
 
 def mxfp4_quantize(x):
@@ -197,7 +201,7 @@ def mxfp4_quantize(x):
         raise ValueError(f"mxfp4_quantize needs bf16, fp16 or fp32, got {x.dtype}")
     if x.dim() < 1:
         raise ValueError("mxfp4_quantize needs at least one dimension")
-    _mx_gpu(x, "mxfp4_quantize")
+    index = _mx_gpu(x, "mxfp4_quantize")
     *lead, K = x.shape
     nb = -(-K // MXFP4_BLOCK)
     if len(lead) == 1 and nb:   # strides given: a quarter of a microsecond sooner each
@@ -216,7 +220,7 @@ def mxfp4_quantize(x):
     if K > 1 and step != 1 and row_step != 1:   # neither rows nor columns in one piece each
         x2 = x2.contiguous()
         row_step, step = K, 1
-    _mx_launch(x2, "mxfp4_quantize", load().kamd_mxfp4_quantize_launch, x2.data_ptr(), q.data_ptr(), scale.data_ptr(),
+    _mx_launch(index, "mxfp4_quantize", load().kamd_mxfp4_quantize_launch, x2.data_ptr(), q.data_ptr(), scale.data_ptr(),
                x2.shape[0], K, row_step, step, code)
     return q, scale
 
@@ -235,14 +239,14 @@ def mxfp4_dequantize(q, scale, k=None, dtype=None):
     k = MXFP4_BLOCK * nb if k is None else int(k)
     if k < 0 or -(-k // MXFP4_BLOCK) != nb:
         raise ValueError(f"mxfp4_dequantize: k={k} does not have {nb} blocks of {MXFP4_BLOCK}")
-    _mx_gpu(q, "mxfp4_dequantize")
+    index = _mx_gpu(q, "mxfp4_dequantize")
     if len(lead) == 1 and k:
         x = torch.empty_strided((lead[0], k), (k, 1), dtype=dtype, device=q.device)
     else:
         x = q.new_empty((*lead, k), dtype=dtype)
     if k == 0 or 0 in lead:
         return x
-    _mx_launch(q, "mxfp4_dequantize", load().kamd_mxfp4_dequantize_launch, q.data_ptr(), scale.data_ptr(), x.data_ptr(),
+    _mx_launch(index, "mxfp4_dequantize", load().kamd_mxfp4_dequantize_launch, q.data_ptr(), scale.data_ptr(), x.data_ptr(),
                scale.numel() // nb, k, code)
     return x
 
@@ -255,17 +259,18 @@ def gemm_mxfp4_nt(a, a_scale, b, b_scale, out_fp32=True, alpha=1.0):
     sa, sb = a.shape, b.shape
     if len(sa) != 2 or len(sb) != 2 or sa[1] != sb[1]:
         raise ValueError(f"gemm_mxfp4_nt needs codes [M, 16 * blocks] and [N, 16 * blocks], got {tuple(sa)} and {tuple(sb)}")
-    if a.device != b.device:
+    if a.get_device() != b.get_device():
         raise ValueError(f"gemm_mxfp4_nt: a on {a.device}, b on {b.device}")
     a, a_scale = _mx_pair(a, a_scale, "gemm_mxfp4_nt a")
     b, b_scale = _mx_pair(b, b_scale, "gemm_mxfp4_nt b")
-    _mx_gpu(a, "gemm_mxfp4_nt")
+    index = _mx_gpu(a, "gemm_mxfp4_nt")
     M, N, nb = sa[0], sb[0], sa[1] // 16
     L = load()
     out = torch.empty_strided((M, N), (N or 1, 1), dtype=torch.float32 if out_fp32 else torch.bfloat16, device=a.device)
-    need = L.kamd_gemm_mxfp4_nt_workspace(M, N, nb) if nb > 1024 or (M > 16 and N > 16) else 0   # few rows: of a long K only
-    ws = a.new_empty(need) if need else None
-    _mx_launch(a, "gemm_mxfp4_nt", L.kamd_gemm_mxfp4_nt_launch, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
+    # none for few rows, but of a long K
+    need = L.kamd_gemm_mxfp4_nt_workspace(M, N, nb) if nb > 500 or (M >= 256 and N >= 256) else 0
+    ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
+    _mx_launch(index, "gemm_mxfp4_nt", L.kamd_gemm_mxfp4_nt_launch, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
                b_scale.data_ptr(), out.data_ptr(), M, N, nb, float(alpha), 1 if out_fp32 else 0,
                ws.data_ptr() if need else None, need)
     return out

@@ -631,6 +631,11 @@ def test_c_entries_refuse_bad_sizes():
     assert gemm(None, None, None, None, None, 0, 1, 1, 1.0, 1, None, 0, None) == 0
     refuses(gemm(p, p, p, p, p, 64, 64, 1024, 1.0, 1, None, 0, None), b"workspace")
     refuses(gemm(p, p, p, p, p, 1, 64, 4096, 1.0, 1, p, 64 * 4, None), b"workspace")
+    # where gemm_mxfp4_nt does not ask, none is needed
+    for few in (1, 16, 17, 63, 64, 100, 255):
+        for many in (1, 64, 255, 256, 1000, 5000, 100000):
+            for nb in (1, 7, 8, 63, 256, 500):
+                assert L.kamd_gemm_mxfp4_nt_workspace(few, many, nb) == L.kamd_gemm_mxfp4_nt_workspace(many, few, nb) == 0
     need = L.kamd_gemm_mxfp4_nt_workspace(8192, 8192, 256)
     assert need >= 2 * 8192 * 256 and L.kamd_gemm_mxfp4_nt_workspace(1, 8192, 256) == 0
     assert L.kamd_gemm_mxfp4_nt_workspace(-5, 8192, 256) == 0 and L.kamd_gemm_mxfp4_nt_workspace(0, 0, 0) == 0
