@@ -759,10 +759,11 @@ gemm_large_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ B, 
     for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // Step s on one set: 64 products, and behind product p ask(p) asks for something. Asked for before the first product,
-  // it would be in what that product waits for.
+  // it would be in what that product waits for. From one product to the next one operand stays, also where a row of
+  // them ends (8192^3: 256.3 -> 254.3 us, for what the change of an operand costs in power).
   auto step = [&](auto s, auto ask) {
     unroll<64>([&](auto p) {
-      constexpr int i = p / 8, j = p % 8;
+      constexpr int i = p / 8, j = i % 2 ? 7 - p % 8 : p % 8;
       mfma16<j % 2 * 2 + s, i % 2 * 2 + s>(acc[i][j], f[s].b[j], f[s].a[i], sc.b[j / 2], sc.a[i / 2]);
       __builtin_amdgcn_sched_barrier(0);
       ask(p);
