@@ -64,7 +64,8 @@ def targets():
                          cxx + ["-shared", "-Wextra", "-Werror", _s("runc", "kamd_devshim.cc"), "-ldl"]),
         "orphan": ([_s("pause", "orphan.cc")], os.path.join(BIN_DIR, "orphan"),
                    ["g++", "-Os", "-Wall", _s("pause", "orphan.cc")]),
-        "kamd_hip": ([_s("hip", "kamd_hip.hip"), _s("hip", "kamd_mxfp4.hip"), _s("hip", "kamd_hip_err.h")],
+        "kamd_hip": ([_s("hip", "kamd_hip.hip"), _s("hip", "kamd_mxfp4.hip"), _s("hip", "kamd_hip_err.h"),
+                      _s("hip", "kamd_diag.h")],
                      os.path.join(LIB_DIR, "libkamd_hip.so"),
                      hip + ["-shared", _s("hip", "kamd_hip.hip"), _s("hip", "kamd_mxfp4.hip")]),
         "hip_vector_add": ([_s("hip", "vector_add_main.hip"), _s("hip", "kamd_hip.hip"), _s("hip", "kamd_hip_err.h")],

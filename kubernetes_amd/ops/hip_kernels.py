@@ -53,6 +53,7 @@ def load():
         L.kamd_diag_mfma.argtypes = [i, i, i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]
         L.kamd_diag_mfma_fp8.argtypes = [i, i, i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]
         L.kamd_diag_mfma_fp4.argtypes = [i, i, i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]
+        L.kamd_diag_mfma_fp4_sample.argtypes = [vp, vp, vp, vp, vp, vp, i, f, ctypes.POINTER(ctypes.c_double)]
         L.kamd_diag_hbm.argtypes = [i, sz, i, ctypes.POINTER(ctypes.c_double)]
         L.kamd_payload_create.argtypes = [i, i]
         L.kamd_payload_create.restype = vp
@@ -322,7 +323,7 @@ def diag_mfma_fp8(dev=0, size=8192, iters=10):
 
 def diag_mfma_fp4(dev=0, size=8192, iters=10):
     """Quantises random bf16 operands to microscaled fp4 and multiplies them; a code or scale that is not the
-    definition's makes `max_rel_err` 1."""
+    definition's makes `max_rel_err` 1, an output that is NaN makes it infinite."""
     tf, err = ctypes.c_double(), ctypes.c_double()
     _raise(load().kamd_diag_mfma_fp4(dev, size, iters, ctypes.byref(tf), ctypes.byref(err)), "diag_mfma_fp4")
     return {"tflops": tf.value, "max_rel_err": err.value, "size": size, "iters": iters}

@@ -16,6 +16,7 @@
 #include <utility>
 #include <vector>
 
+#include "kamd_diag.h"
 #include "kamd_hip_err.h"
 
 #define HC(x)                                 \
@@ -1296,10 +1297,51 @@ int kamd_gemm_mxfp4_nt_launch(const void* A, const void* As, const void* B, cons
                   : mxfp4::launch_gemm<__bf16>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);
 }
 
+// One sampled output of the fp4 burn-in, on the host: `got` = row A times row B, each row with its `size` bf16 values, codes
+// and scales. Codes and scales have to be the definition's (else the error is 1), and `got` is held against the product of
+// the codes in 64 bits, relative to the sum of magnitudes. *worst becomes the worse of itself and these.
+int kamd_diag_mfma_fp4_sample(const uint16_t* xa, const uint8_t* qa, const uint8_t* sa, const uint16_t* xb, const uint8_t* qb,
+                              const uint8_t* sb, int size, float got, double* worst) {
+  if (size < 32 || size % 32 || !xa || !qa || !sa || !xb || !qb || !sb || !worst) return kamd_fail("diag_mfma_fp4_sample: bad arguments");
+  static const double grid[8] = {0, 0.5, 1, 1.5, 2, 3, 4, 6};
+  bool exact = true;
+  auto block = [&](const uint16_t* x, const uint8_t* q, int scale, double* v) {   // the values of 32 codes
+    double in[32], top = 0;
+    bool finite = true;
+    for (int k = 0; k < 32; ++k) {
+      const uint32_t u = (uint32_t)x[k] << 16;
+      float f;
+      memcpy(&f, &u, 4);
+      in[k] = f;
+      finite &= std::isfinite(f);
+      if (fabs(in[k]) > top) top = fabs(in[k]);
+    }
+    const int s = !finite ? 255 : top == 0 || ilogb(top) < 2 - 127 ? 0 : ilogb(top) - 2 + 127;
+    exact &= s == scale;
+    for (int k = 0; k < 32; ++k) {
+      const int code = (q[k / 2] >> (k % 2 * 4)) & 15;
+      const double w = fabs(ldexp(in[k], 127 - s));
+      const int want = (w > 0.25) + (w >= 0.75) + (w > 1.25) + (w >= 1.75) + (w > 2.5) + (w >= 3.5) + (w > 5) + (std::signbit(in[k]) ? 8 : 0);
+      exact &= code == (finite ? want : 0);
+      v[k] = scale == 255 ? NAN : ldexp(code & 8 ? -grid[code & 7] : grid[code & 7], scale - 127);
+    }
+  };
+  double ref = 0, mag = 0;
+  for (int b = 0; b < size / 32; ++b) {
+    double va[32], vb[32];
+    block(xa + b * 32, qa + b * 16, sa[b], va);
+    block(xb + b * 32, qb + b * 16, sb[b], vb);
+    for (int k = 0; k < 32; ++k) {
+      ref += va[k] * vb[k];
+      mag += fabs(va[k] * vb[k]);
+    }
+  }
+  *worst = kamd_worse(kamd_worse(*worst, exact ? 0 : 1), fabs(got - ref) / (mag > 1e-30 ? mag : 1.0));
+  return 0;
+}
+
 // fp4 burn-in, the protocol of kamd_diag_mfma: random bf16 operands of size x size are quantised on the device, then
-// `iters` products timed. Sampled rows are checked on the host: their codes and scales against the definition, which
-// they have to meet exactly (else the error is 1), and outputs against a product of the codes in 64 bits, relative
-// to the sum of magnitudes. size is a multiple of 32.
+// `iters` products timed, and 256 outputs checked with their rows. size is a multiple of 32.
 int kamd_diag_mfma_fp4(int dev, int size, int iters, double* tflops, double* max_rel_err) {
   using namespace mxfp4;
   if (size < 32 || size % 32 || iters < 1)
@@ -1337,48 +1379,24 @@ int kamd_diag_mfma_fp4(int dev, int size, int iters, double* tflops, double* max
       *tflops = 2.0 * size * size * (double)size * iters / (ms * 1e-3) / 1e12;
 
       double worst = 0;
-      std::vector<uint16_t> hx(n);
-      std::vector<uint8_t> hq(n / 2), hs(nb);
-      std::vector<double> va(n), vb(n);
-      auto fetch = [&](const uint16_t* rx, const uint8_t* rq, const uint8_t* rs, std::vector<double>& v) {
-        if (kamd_check(hipMemcpy(hx.data(), rx, n * 2, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") != 0 ||
-            kamd_check(hipMemcpy(hq.data(), rq, n / 2, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") != 0 ||
-            kamd_check(hipMemcpy(hs.data(), rs, nb, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") != 0)
-          return false;
-        static const double grid[8] = {0, 0.5, 1, 1.5, 2, 3, 4, 6};
-        for (size_t b = 0; b < nb; ++b) {
-          double in[32], top = 0;
-          for (int k = 0; k < 32; ++k) {
-            const uint32_t u = (uint32_t)hx[b * 32 + k] << 16;
-            float f;
-            memcpy(&f, &u, 4);
-            in[k] = f;
-            if (fabs(in[k]) > top) top = fabs(in[k]);
-          }
-          const int s = top == 0 ? 0 : ilogb(top) - 2 + 127;
-          if (s != hs[b]) worst = 1;
-          for (int k = 0; k < 32; ++k) {
-            const double w = fabs(ldexp(in[k], 127 - s));
-            const int want = (w > 0.25) + (w >= 0.75) + (w > 1.25) + (w >= 1.75) + (w > 2.5) + (w >= 3.5) + (w > 5);
-            const int code = (hq[(b * 32 + k) / 2] >> (k % 2 * 4)) & 15;
-            if ((code & 7) != want || (code >= 8) != std::signbit(in[k])) worst = 1;
-            v[b * 32 + k] = ldexp(code & 8 ? -grid[code & 7] : grid[code & 7], hs[b] - 127);
-          }
-        }
-        return true;
+      struct Row {
+        std::vector<uint16_t> x;
+        std::vector<uint8_t> q, s;
+      } a, b;
+      auto fetch = [&](Row& to, const uint16_t* x, const uint8_t* q, const uint8_t* s) {
+        to.x.resize(n);
+        to.q.resize(n / 2);
+        to.s.resize(nb);
+        return kamd_check(hipMemcpy(to.x.data(), x, n * 2, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") == 0 &&
+               kamd_check(hipMemcpy(to.q.data(), q, n / 2, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") == 0 &&
+               kamd_check(hipMemcpy(to.s.data(), s, nb, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") == 0;
       };
       for (int t = 0; t < 256 && ok; ++t) {
         const size_t i = (size_t)t * 7919u % n, j = ((size_t)t * 104729u + 13u) % n;
         float got = 0;
-        ok = fetch(x + i * n, qa + i * n / 2, sa + i * nb, va) && fetch(x + (n + j) * n, qb + j * n / 2, sb + j * nb, vb) &&
-             kamd_check(hipMemcpy(&got, c + i * n + j, 4, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") == 0;
-        double ref = 0, mag = 0;
-        for (size_t k = 0; k < n; ++k) {
-          ref += va[k] * vb[k];
-          mag += fabs(va[k] * vb[k]);
-        }
-        const double err = fabs(got - ref) / (mag > 1e-30 ? mag : 1.0);
-        if (!(err <= worst)) worst = err;   // a NaN as well
+        ok = fetch(a, x + i * n, qa + i * n / 2, sa + i * nb) && fetch(b, x + (n + j) * n, qb + j * n / 2, sb + j * nb) &&
+             kamd_check(hipMemcpy(&got, c + i * n + j, 4, hipMemcpyDeviceToHost), "diag_mfma_fp4 copy") == 0 &&
+             kamd_diag_mfma_fp4_sample(a.x.data(), a.q.data(), a.s.data(), b.x.data(), b.q.data(), b.s.data(), size, got, &worst) == 0;
       }
       if (!ok) break;
       *max_rel_err = worst;
