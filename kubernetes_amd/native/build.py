@@ -68,7 +68,8 @@ def targets():
                       _s("hip", "kamd_diag.h")],
                      os.path.join(LIB_DIR, "libkamd_hip.so"),
                      hip + ["-shared", _s("hip", "kamd_hip.hip"), _s("hip", "kamd_mxfp4.hip")]),
-        "hip_vector_add": ([_s("hip", "vector_add_main.hip"), _s("hip", "kamd_hip.hip"), _s("hip", "kamd_hip_err.h")],
+        "hip_vector_add": ([_s("hip", "vector_add_main.hip"), _s("hip", "kamd_hip.hip"), _s("hip", "kamd_hip_err.h"),
+                            _s("hip", "kamd_diag.h")],
                            os.path.join(BIN_DIR, "hip-vector-add"),
                            hip + [_s("hip", "vector_add_main.hip"), _s("hip", "kamd_hip.hip")]),
         "xgmi_probe": ([_s("hip", "xgmi_probe.cc")], os.path.join(BIN_DIR, "xgmi-probe"),

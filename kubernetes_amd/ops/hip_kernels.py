@@ -53,6 +53,10 @@ def load():
         L.kamd_diag_mfma.argtypes = [i, i, i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]
         L.kamd_diag_mfma_fp8.argtypes = [i, i, i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]
         L.kamd_diag_mfma_fp4.argtypes = [i, i, i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]
+        L.kamd_diag_vector_add_error.argtypes = [vp, vp, vp, i]
+        L.kamd_diag_vector_add_error.restype = f
+        L.kamd_diag_mfma_sample.argtypes = [vp, vp, i, i, f, ctypes.POINTER(ctypes.c_double)]
+        L.kamd_diag_mfma_sample.restype = None
         L.kamd_diag_mfma_fp4_sample.argtypes = [vp, vp, vp, vp, vp, vp, i, f, ctypes.POINTER(ctypes.c_double)]
         L.kamd_diag_hbm.argtypes = [i, sz, i, ctypes.POINTER(ctypes.c_double)]
         L.kamd_payload_create.argtypes = [i, i]

@@ -22,6 +22,7 @@
 
 #include <vector>
 
+#include "kamd_diag.h"
 #include "kamd_hip_err.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -1033,6 +1034,32 @@ void kamd_hbm_copy_config(int variant, int blocks) {
 // --- self-contained diagnostics (allocate, run, verify, free) -------------
 
 // vectorAdd sample semantics: returns 0 and prints nothing; *max_err = max |c - (a+b)|.
+// The largest error of c = a + b, on the host.
+float kamd_diag_vector_add_error(const float* a, const float* b, const float* c, int n) {
+  double worst = 0;
+  for (int i = 0; i < n; ++i) worst = kamd_worse(worst, fabsf(c[i] - (a[i] + b[i])));
+  return (float)worst;
+}
+
+// One sampled output of the bf16 or fp8 (e4m3) burn-in, on the host: `got` against row A times row B of K values in 64 bits,
+// relative to the sum of magnitudes. *worst becomes the worse of itself and that.
+void kamd_diag_mfma_sample(const void* a, const void* b, int K, int fp8, float got, double* worst) {
+  auto value = [&](const void* p, int k) {
+    if (fp8) return fp8_e4m3_to_double(((const unsigned char*)p)[k]);
+    const uint32_t u = (uint32_t)((const u16*)p)[k] << 16;
+    float f;
+    memcpy(&f, &u, 4);
+    return (double)f;
+  };
+  double ref = 0, mag = 0;
+  for (int k = 0; k < K; ++k) {
+    const double p = value(a, k) * value(b, k);
+    ref += p;
+    mag += fabs(p);
+  }
+  *worst = kamd_worse(*worst, fabs(got - ref) / (mag > 1e-30 ? mag : 1.0));
+}
+
 int kamd_diag_vector_add(int dev, int n, float* max_err) {
   HC(hipSetDevice(dev));
   std::vector<float> ha(n), hb(n), hc(n);
@@ -1050,13 +1077,7 @@ int kamd_diag_vector_add(int dev, int n, float* max_err) {
   hipLaunchKernelGGL(vector_add_kernel, dim3((n + 255) / 256), dim3(256), 0, 0, da, db, dc, n);
   HC(hipGetLastError());
   HC(hipMemcpy(hc.data(), dc, bytes, hipMemcpyDeviceToHost));
-  float e = 0.f;
-  for (int i = 0; i < n; ++i) {
-    float d = hc[i] - (ha[i] + hb[i]);
-    if (d < 0) d = -d;
-    if (d > e) e = d;
-  }
-  *max_err = e;
+  *max_err = kamd_diag_vector_add_error(ha.data(), hb.data(), hc.data(), n);
   hipFree(da);
   hipFree(db);
   hipFree(dc);
@@ -1098,16 +1119,7 @@ int kamd_diag_mfma_fp8(int dev, int size, int iters, double* tflops, double* max
     double worst = 0;
     for (int s = 0; s < 256; ++s) {
       int i = (int)((s * 7919u) % (unsigned)M), j = (int)((s * 104729u + 13u) % (unsigned)N);
-      double ref = 0, mag = 0;
-      for (int k = 0; k < K; ++k) {
-        double pr = fp8_e4m3_to_double(ha[(size_t)i * K + k]) * fp8_e4m3_to_double(hb[(size_t)j * K + k]);
-        ref += pr;
-        mag += pr < 0 ? -pr : pr;
-      }
-      double err = hc[(size_t)i * N + j] - ref;
-      if (err < 0) err = -err;
-      double rel = err / (mag > 1e-30 ? mag : 1.0);
-      if (rel > worst) worst = rel;
+      kamd_diag_mfma_sample(&ha[(size_t)i * K], &hb[(size_t)j * K], K, 1, hc[(size_t)i * N + j], &worst);
     }
     *max_rel_err = worst;
     rc = 0;
@@ -1151,20 +1163,10 @@ int kamd_diag_mfma(int dev, int size, int iters, double* tflops, double* max_rel
   HC(hipMemcpy(ha.data(), A, ha.size() * 2, hipMemcpyDeviceToHost));
   HC(hipMemcpy(hb.data(), B, hb.size() * 2, hipMemcpyDeviceToHost));
   HC(hipMemcpy(hc.data(), C, hc.size() * 4, hipMemcpyDeviceToHost));
-  auto bf = [](u16 v) { uint32_t u = (uint32_t)v << 16; float f; memcpy(&f, &u, 4); return (double)f; };
   double worst = 0;
   for (int s = 0; s < 256; ++s) {
     int i = (int)((s * 7919u) % (unsigned)M), j = (int)((s * 104729u + 13u) % (unsigned)N);
-    double ref = 0, mag = 0;
-    for (int k = 0; k < K; ++k) {
-      double p = bf(ha[(size_t)i * K + k]) * bf(hb[(size_t)j * K + k]);
-      ref += p;
-      mag += p < 0 ? -p : p;
-    }
-    double err = hc[(size_t)i * N + j] - ref;
-    if (err < 0) err = -err;
-    double rel = err / (mag > 1e-30 ? mag : 1.0);
-    if (rel > worst) worst = rel;
+    kamd_diag_mfma_sample(&ha[(size_t)i * K], &hb[(size_t)j * K], K, 0, hc[(size_t)i * N + j], &worst);
   }
   *max_rel_err = worst;
   hipEventDestroy(e0);

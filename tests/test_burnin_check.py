@@ -115,3 +115,51 @@ def test_sample_refuses_sizes(lib):
     for size in (0, -32, 31, 33):
         assert lib.kamd_diag_mfma_fp4_sample(*args, size, 0.0, ctypes.byref(worst)) == -1
     assert lib.kamd_diag_mfma_fp4_sample(None, *args[1:], SIZE, 0.0, ctypes.byref(worst)) == -1 and worst.value == 0
+
+
+# ---------------------------------------------------------------------------
+# the bf16 and fp8 products and vector_add
+
+def wide_row(seed, fp8):
+    """Bits of SIZE values and the values."""
+    r = np.random.default_rng(seed)
+    if fp8:   # e4m3: the codes of 1.0 to 1.875 and their negatives
+        bits = (0x38 + r.integers(0, 8, SIZE) + 0x80 * r.integers(0, 2, SIZE)).astype(np.uint8)
+        return bits, (1 + (bits & 7) / 8.0) * np.where(bits & 0x80, -1, 1)
+    bits = (r.uniform(-1, 1, SIZE).astype(np.float32).view(np.uint32) >> 16).astype(np.uint16)
+    return bits, (bits.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+
+
+@pytest.mark.parametrize("at", [0, 4, 8, None])
+@pytest.mark.parametrize("wrong_output", [NAN, INF, -INF, 1e6])
+@pytest.mark.parametrize("fp8", [0, 1])
+def test_wide_sample(lib, fp8, wrong_output, at):
+    worst = ctypes.c_double(0)
+    for seed in range(9):
+        (a, va), (b, vb) = wide_row(seed, fp8), wide_row(100 + seed, fp8)
+        got = wrong_output if seed == at else float(va @ vb)
+        lib.kamd_diag_mfma_sample(a.ctypes.data_as(ctypes.c_void_p), b.ctypes.data_as(ctypes.c_void_p), SIZE, fp8, got,
+                                  ctypes.byref(worst))
+    if at is None:
+        assert worst.value <= 2.0 ** -24
+    else:
+        assert worst.value == INF if wrong_output != 1e6 else 1e3 < worst.value < 1e6
+        r = BurnInResult(ok=False, tflops=1400.0, hbm_gbps=6000.0, fp8_tflops=2800.0)
+        r.mfma_rel_err, r.fp8_rel_err = (0.0, worst.value) if fp8 else (worst.value, 0.0)
+        assert "relative error" in BurnIn().judge(r)
+
+
+@pytest.mark.parametrize("at", [0, 500, 999, None])
+@pytest.mark.parametrize("wrong_output", [NAN, INF, 1e6])
+def test_vector_add_error(lib, wrong_output, at):
+    r = np.random.default_rng(1)
+    a, b = r.uniform(0, 1, 1000).astype(np.float32), r.uniform(0, 1, 1000).astype(np.float32)
+    c = a + b
+    if at is not None:
+        c[at] = wrong_output
+    got = lib.kamd_diag_vector_add_error(*(v.ctypes.data_as(ctypes.c_void_p) for v in (a, b, c)), 1000)
+    if at is None:
+        assert got == 0
+    else:
+        assert got == INF if wrong_output != 1e6 else got > 1e5
+        assert "vector_add" in BurnIn().judge(BurnInResult(ok=False, vadd_err=got, tflops=1400.0, hbm_gbps=6000.0, fp8_tflops=2800.0))
