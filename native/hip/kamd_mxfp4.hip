@@ -149,15 +149,15 @@ quantize_rows_kernel(const void* __restrict__ xv, uint32_t* __restrict__ q, uint
 // through LDS, so that whole cache lines are written. Rows of memory and columns behind the last read as 0.
 template <int TYPE>
 __global__ void __launch_bounds__(512)
-quantize_cols_kernel(const void* __restrict__ xv, uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int64_t M, int64_t K,
-                     int64_t ld, int64_t nb) {
+quantize_cols_kernel(const void* __restrict__ xv, uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int64_t first, int64_t M,
+                     int64_t K, int64_t ld, int64_t nb) {
   typedef typename Elem<TYPE>::bits bits;
   constexpr int COLS = TYPE == FP32 ? 1 : 2, ROWS = 64 * COLS, PITCH = 128 + 16;
   __shared__ __attribute__((aligned(16))) uint8_t codes[ROWS * PITCH];
   __shared__ __attribute__((aligned(8))) uint8_t scales[ROWS * 8];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t tiles_m = (M + ROWS - 1) / ROWS;
-  const int64_t m0 = (int64_t)blockIdx.x % tiles_m * ROWS, b0 = (int64_t)blockIdx.x / tiles_m * 8;
+  const int64_t tiles_m = (M + ROWS - 1) / ROWS, tile = first + blockIdx.x;
+  const int64_t m0 = tile % tiles_m * ROWS, b0 = tile / tiles_m * 8;
   const int64_t m = m0 + lane * COLS;
   {
     const int b = wave;
@@ -1035,8 +1035,19 @@ __global__ void __launch_bounds__(256) fill_kernel(uint16_t* __restrict__ x, siz
   }
 }
 
-// A launch's workgroups times 256 lanes stay below 2^32; longer runs take several launches.
+// A launch's lanes stay below 2^32; longer runs take several launches.
 constexpr size_t SLICE = (size_t)1 << 31;
+// An item's place in its row has 32 bits in the kernels. A longer row is taken in pieces of this many values; its codes, its
+// scales and what they stand for are one run each. No memory holds the codes of a row of LONGEST.
+constexpr int64_t ROW_ITEMS = (int64_t)1 << 31, PIECE = (int64_t)1 << 32, LONGEST = (int64_t)1 << 39;
+
+template <typename F>
+static int pieces(int64_t rows, int64_t K, F launch) {
+  for (int64_t r = 0; r < rows; ++r)
+    for (int64_t k = 0; k < K; k += PIECE)
+      if (launch(r, k, K - k < PIECE ? K - k : PIECE) != 0) return -1;
+  return 0;
+}
 
 template <typename F>
 static int sliced(size_t items, F launch) {
@@ -1232,17 +1243,25 @@ int kamd_mxfp4_quantize_launch(const void* x, void* q, void* scale, int64_t rows
   if (rows < 0 || K < 0 || type < 0 || type > 2 || (step != 1 && row_step != 1 && K > 1))
     return kamd_fail("mxfp4_quantize: bad arguments");
   if (rows == 0 || K == 0) return 0;
+  if (K >= LONGEST) return kamd_fail("mxfp4_quantize: K (%lld) is too large", (long long)K);
   const int64_t nb = (K + 31) / 32, row_items = nb * 4;
-  if (row_items >= (int64_t)1 << 31) return kamd_fail("mxfp4_quantize: K (%lld) is too large", (long long)K);
   if (!x || !q || !scale) return kamd_fail("mxfp4_quantize: a null pointer");
   if (((uintptr_t)q) & 15) return kamd_fail("mxfp4_quantize: codes must be 16-byte aligned");
   if (step != 1 && K > 1) {
-    const int64_t tile = type == FP32 ? 64 : 128, tiles = (rows + tile - 1) / tile * ((nb + 7) / 8);
-    if (tiles >= (int64_t)1 << 23) return kamd_fail("mxfp4_quantize: %lld x %lld is too large", (long long)rows, (long long)K);
+    const int64_t tile = type == FP32 ? 64 : 128, tiles = (rows + tile - 1) / tile * ((nb + 7) / 8), most = SLICE / 512;
     auto k = type == BF16 ? quantize_cols_kernel<BF16> : type == FP16 ? quantize_cols_kernel<FP16> : quantize_cols_kernel<FP32>;
-    hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(512), 0, stream, x, (uint8_t*)q, (uint8_t*)scale, rows, K, step, nb);
-    return kamd_check(hipGetLastError(), "mxfp4_quantize launch");
+    for (int64_t first = 0; first < tiles; first += most) {
+      hipLaunchKernelGGL(k, dim3((unsigned)(tiles - first < most ? tiles - first : most)), dim3(512), 0, stream, x, (uint8_t*)q,
+                         (uint8_t*)scale, first, rows, K, step, nb);
+      HC(hipGetLastError());
+    }
+    return 0;
   }
+  if (row_items >= ROW_ITEMS)
+    return pieces(rows, K, [&](int64_t r, int64_t k, int64_t n) {
+      return kamd_mxfp4_quantize_launch((const char*)x + (r * row_step + k) * (type == FP32 ? 4 : 2), (char*)q + r * nb * 16 + k / 2,
+                                        (char*)scale + r * nb + k / 32, 1, n, n, 1, type, stream);
+    });
   const size_t items = (size_t)rows * row_items;
   return sliced(items, [&](size_t first, dim3 grid) {
     auto k = type == BF16 ? quantize_rows_kernel<BF16> : type == FP16 ? quantize_rows_kernel<FP16> : quantize_rows_kernel<FP32>;
@@ -1257,10 +1276,15 @@ int kamd_mxfp4_dequantize_launch(const void* q, const void* scale, void* x, int6
   using namespace mxfp4;
   if (rows < 0 || K < 0 || type < 0 || type > 2) return kamd_fail("mxfp4_dequantize: bad arguments");
   if (rows == 0 || K == 0) return 0;
-  const int64_t row_items = (K + 31) / 32 * (type == FP32 ? 8 : 4);
-  if (row_items >= (int64_t)1 << 31) return kamd_fail("mxfp4_dequantize: K (%lld) is too large", (long long)K);
+  if (K >= LONGEST) return kamd_fail("mxfp4_dequantize: K (%lld) is too large", (long long)K);
+  const int64_t nb = (K + 31) / 32, row_items = nb * (type == FP32 ? 8 : 4);
   if (!q || !scale || !x) return kamd_fail("mxfp4_dequantize: a null pointer");
   if (((uintptr_t)q) & 3) return kamd_fail("mxfp4_dequantize: codes must be 4-byte aligned");
+  if (row_items >= ROW_ITEMS)
+    return pieces(rows, K, [&](int64_t r, int64_t k, int64_t n) {
+      return kamd_mxfp4_dequantize_launch((const char*)q + r * nb * 16 + k / 2, (const char*)scale + r * nb + k / 32,
+                                          (char*)x + (r * K + k) * (type == FP32 ? 4 : 2), 1, n, type, stream);
+    });
   const size_t items = (size_t)rows * row_items;
   const bool stream_out = K * (type == FP32 ? 4 : 2) % 16 == 0 && ((uintptr_t)x & 15) == 0;
   return sliced(items, [&](size_t first, dim3 grid) {

@@ -1,0 +1,112 @@
+"""Microscaled fp4 at sizes that one launch does not hold: rows of more than 2^34 values, tall transposed views. Values and
+codes are equal, as in the tests of ordinary sizes; between a few written places everything is zero and has to stay so."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from kubernetes_amd.ops import hip_kernels as hk  # noqa: E402
+from test_mxfp4 import operand, quantized, values_of  # noqa: E402
+
+
+@pytest.fixture
+def gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    hk.load()   # must load: no fallback
+    yield torch.device("cuda")
+    torch.cuda.empty_cache()
+
+
+def places(K, edges):
+    """Blocks to write around these values of a row and at its ends, as (first, behind the last)."""
+    nb = -(-K // 32)
+    return [(max(e // 32 - 2, 0), min(e // 32 + 2, nb)) for e in (0, *edges, K)]
+
+
+def write(x, at, K, seed):
+    """Random values at these blocks of each row of x; their codes and scales."""
+    g = torch.Generator().manual_seed(seed)
+    want = []
+    for lo, hi in at:
+        v = torch.randn(x.shape[0], min(hi * 32, K) - lo * 32, generator=g).to(x.dtype)
+        x[:, lo * 32:lo * 32 + v.shape[1]] = v.to(x.device)
+        want.append(quantized(v))
+    return want
+
+
+def nonzero(t):
+    """How many are not zero, in pieces: counted at once, a tensor of this size needs several times its memory."""
+    return sum(p.count_nonzero().item() for p in t.view(-1).split(1 << 28))
+
+
+def check(q, s, at, want):
+    for (lo, hi), (want_q, want_s) in zip(at, want):
+        assert torch.equal(q[:, lo * 16:hi * 16].cpu(), want_q) and torch.equal(s[:, lo:hi].cpu(), want_s)
+    assert nonzero(q) == sum(w.count_nonzero().item() for w, _ in want)
+    assert nonzero(s) == sum(w.count_nonzero().item() for _, w in want)
+
+
+@pytest.mark.gpu
+def test_quantize_and_dequantize_long_rows(gpu):
+    rows, K = 2, (1 << 34) + 37
+    at = places(K, [1 << 32, 1 << 33, 3 << 32, 1 << 34])[:-1]
+    x = torch.zeros(rows, K, device=gpu, dtype=torch.bfloat16)
+    want = write(x, at, K, 1)
+    q, s = hk.mxfp4_quantize(x)
+    check(q, s, at, want)
+    q1, s1 = hk.mxfp4_quantize(x[1])     # one dimension, and an odd start
+    assert torch.equal(q1, q[1]) and torch.equal(s1, s[1])
+    del q1, s1
+    x.fill_(1.0)
+    y = hk.mxfp4_dequantize(q, s, k=K)
+    total = 0
+    for (lo, hi), (want_q, want_s) in zip(at, want):
+        v = values_of(want_q, want_s)[:, :min(hi * 32, K) - lo * 32]
+        assert torch.equal(y[:, lo * 32:lo * 32 + v.shape[1]].cpu().double(), v)
+        total += v.count_nonzero().item()
+    assert nonzero(y) == total
+
+
+@pytest.mark.gpu
+def test_dequantize_long_row_to_fp32(gpu):
+    K = (1 << 33) + 5
+    nb = -(-K // 32)
+    q = torch.zeros(1, 16 * nb, device=gpu, dtype=torch.uint8)
+    s = torch.full((1, nb), 127, device=gpu, dtype=torch.uint8)
+    at = places(K, [1 << 31, 1 << 32])
+    for i, (lo, hi) in enumerate(at):
+        q[:, lo * 16:hi * 16] = operand(1, hi - lo, i)[0]
+    y = hk.mxfp4_dequantize(q, s, k=K, dtype=torch.float32)
+    total = 0
+    for lo, hi in at:
+        v = values_of(q[:, lo * 16:hi * 16], s[:, lo:hi])[:, :min(hi * 32, K) - lo * 32]
+        assert torch.equal(y[:, lo * 32:lo * 32 + v.shape[1]].cpu().double(), v)
+        total += v.count_nonzero().item()
+    assert nonzero(y) == total
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantize_tall_transposed_view(gpu, dtype):
+    rows, K = 2, (1 << 31) + 45
+    at = places(K, [1 << 30, (1 << 30) + 4096])
+    at[-1] = (at[-1][0] - 1, -(-K // 32))
+    x = torch.zeros(K, rows, device=gpu, dtype=dtype).t()
+    want = write(x, at, K, 2)
+    q, s = hk.mxfp4_quantize(x)
+    check(q, s, at, want)
+
+
+def test_rows_that_no_memory_holds_are_refused():
+    try:
+        L = hk.load()
+    except hk.HIPError:
+        pytest.skip("the library is not built")
+    p = 4096    # no pointer: every call is refused before one is used
+    for K in (1 << 39, 1 << 62):
+        for rows in (1, 3):
+            for steps in ((K, 1), (1, 2)):
+                assert L.kamd_mxfp4_quantize_launch(p, p, p, rows, K, *steps, 0, None) == -1
+                assert b"too large" in L.kamd_hip_last_error()
+            assert L.kamd_mxfp4_dequantize_launch(p, p, p, rows, K, 2, None) == -1
+            assert b"too large" in L.kamd_hip_last_error()
