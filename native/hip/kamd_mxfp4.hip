@@ -289,8 +289,8 @@ __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__bf16* p, float v) { *p = (__bf16)v; }
 
 template <typename OutT>
-__global__ void __launch_bounds__(256) zero_kernel(OutT* __restrict__ C, size_t n) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+__global__ void __launch_bounds__(256) zero_kernel(OutT* __restrict__ C, size_t first, size_t n) {
+  const size_t i = first + (size_t)blockIdx.x * 256 + threadIdx.x;
   if (i < n) C[i] = (OutT)0.f;
 }
 
@@ -1210,9 +1210,9 @@ static int launch_gemm(const void* A, const void* As, const void* B, const void*
                        float alpha, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   const size_t n = (size_t)M * N;
   if (nb == 0) {
-    if (n > SLICE) return kamd_fail("gemm_mxfp4_nt: an empty K with more than 2^31 outputs");
-    hipLaunchKernelGGL(zero_kernel<OutT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, (OutT*)C, n);
-    return kamd_check(hipGetLastError(), "gemm_mxfp4_nt launch");
+    return sliced(n, [&](size_t first, dim3 grid) {
+      hipLaunchKernelGGL(zero_kernel<OutT>, grid, dim3(256), 0, stream, (OutT*)C, first, n);
+    });
   }
   const int tile = tile_size(M, N, nb);
   if (tile == 256) return launch_large<OutT>(A, As, B, Bs, C, M, N, nb, alpha, workspace, workspace_bytes, stream);

@@ -97,6 +97,21 @@ def test_quantize_tall_transposed_view(gpu, dtype):
     check(q, s, at, want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp32,dtype", [(True, torch.float32), (False, torch.bfloat16)])
+def test_product_over_an_empty_k_behind_32_bits(gpu, fp32, dtype):
+    """More than 2^31 outputs, all of them zeros, over memory that held something else."""
+    M, N = 46400, 46401
+    a, sa = operand(M, 0, 1)
+    b, sb = operand(N, 0, 2)
+    left = torch.full((M, N), 7.0, device=gpu, dtype=dtype)
+    at = left.data_ptr()
+    del left
+    out = hk.gemm_mxfp4_nt(a, sa, b, sb, out_fp32=fp32)
+    assert out.data_ptr() == at and out.shape == (M, N) and out.dtype == dtype
+    assert nonzero(out) == 0
+
+
 def test_rows_that_no_memory_holds_are_refused():
     try:
         L = hk.load()
