@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(256)
 arrange_scales_kernel(const uint8_t* __restrict__ As, const uint8_t* __restrict__ Bs, uint8_t* __restrict__ out, int M, int N,
                       int nb) {
   constexpr int PITCH = 68;   // 17 banks: 16 rows' words of one tile lie in different ones
-  __shared__ uint8_t rows[128 * PITCH];
+  __shared__ __attribute__((aligned(16))) uint8_t rows[128 * PITCH];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int nt = (nb + 7) / 8, t0 = (int)blockIdx.y * 8;
   const int panels_a = (M + 255) / 256 * 2, panel = (int)blockIdx.x;
