@@ -916,6 +916,11 @@ gemm_rows_kernel(const uint8_t* __restrict__ P, const uint8_t* __restrict__ Ps, 
 
   struct Scales { uint32_t v[GROUPS]; };
   auto load = [&](int t, int buffer, Scales& s, auto part) {
+    // The buffer's last reads have returned. Its products, which are behind them, wait for that too, but nothing keeps the
+    // compiler from moving those behind these loads.
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(waitcnt(63, 0));
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) {
       const uint8_t* p = (i < NP ? Ps : Qs) + srow[i] + (size_t)t * 8 + g * 2;
@@ -965,7 +970,7 @@ gemm_rows_kernel(const uint8_t* __restrict__ P, const uint8_t* __restrict__ Ps, 
   constexpr std::integral_constant<int, 0> none{};
   constexpr std::false_type whole{};
   constexpr std::true_type part{};
-  // unit t in one buffer, the wave's next on its way into the other, whose last reads have returned
+  // unit t in one buffer, the wave's next on its way into the other
   Scales s[2];
   auto unit = [&](int t, auto buffer) {
     const bool more = t + WAVES < units;
