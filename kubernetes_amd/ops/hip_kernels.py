@@ -258,8 +258,8 @@ def mxfp4_dequantize(q, scale, k=None, dtype=None):
 
 def gemm_mxfp4_nt(a, a_scale, b, b_scale, out_fp32=True, alpha=1.0):
     """C = alpha * a @ b.T of microscaled fp4 operands as mxfp4_quantize makes them: a [M, 16 * nb], a_scale
-    [M, nb], b [N, 16 * nb], b_scale [N, nb]; sums in fp32, C fp32 or bf16. Any M and N; K is 32 * nb. A block
-    of scale 255 makes every output that it enters NaN. No gradient is recorded."""
+    [M, nb], b [N, 16 * nb], b_scale [N, nb]; sums in fp32, C fp32 or bf16. Any M, N and nb up to 2^27 each; K is
+    32 * nb. A block of scale 255 makes every output that it enters NaN. No gradient is recorded."""
     import torch
     sa, sb = a.shape, b.shape
     if len(sa) != 2 or len(sb) != 2 or sa[1] != sb[1]:

@@ -125,3 +125,16 @@ def test_rows_that_no_memory_holds_are_refused():
                 assert b"too large" in L.kamd_hip_last_error()
             assert L.kamd_mxfp4_dequantize_launch(p, p, p, rows, K, 2, None) == -1
             assert b"too large" in L.kamd_hip_last_error()
+
+
+def test_products_past_the_documented_sizes_are_refused():
+    try:
+        L = hk.load()
+    except hk.HIPError:
+        pytest.skip("the library is not built")
+    p = 4096
+    for at in range(3):
+        sizes = [1, 1, 1]
+        sizes[at] = (1 << 27) + 1
+        assert L.kamd_gemm_mxfp4_nt_launch(p, p, p, p, p, *sizes, 1.0, 1, None, 0, None) == -1
+        assert b"out of range" in L.kamd_hip_last_error()
