@@ -640,8 +640,8 @@ gemm_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ As, 
 // one workgroup, a SIMD one wave, with all 512 registers: 256 of sums, two sets of fragments.
 // At full rate this runs into the card's power, so that what counts is energy: products alone, from registers, of
 // random codes, run at 7.2 PFLOP/s in this form and 6.5 as 32x32x64 (8.3 both, of zeros). 8192^3 takes 252 us to fp32
-// and 232 to bf16 with the scales' launch, 4.4 and 4.7 PFLOP/s, at 1.85 of 2.4 GHz, products in 62 % of the cycles; the
-// rest is the write of C at the end of each of 4 rounds, by all CUs at one time (11 us a round to fp32).
+// and 232 to bf16 with the scales' launch, 4.4 and 4.7 PFLOP/s, at 1.85 of 2.4 GHz, products in 62 % of the cycles; about
+// half of the rest is the write of C at the end of each of 4 rounds, by all CUs at one time (11 us a round to fp32).
 
 // Scales in the order in which the lanes take them: panel (a wave's 128 rows) by tile of K, 64 lanes of 16 bytes, lane
 // (r, g) having the 16 bits of its chunks 2 g and 2 g + 1 of rows r, 16 + r, .. 112 + r. Read where they lie, a row's 8
@@ -883,9 +883,11 @@ gemm_large_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ B, 
 // with the few; a workgroup makes NP x NQ tiles of 16x16 (v_mfma_scale_f32_16x16x128_f8f6f4), its WAVES taking units
 // of 8 blocks (256 values, 128 B a row) of K in turn, each through two buffers of its own in LDS: no wave waits for
 // another before the sums meet, in the order of the waves. (Straight to registers the instruction's layout has
-// neighbouring lanes read different rows, 16 bytes of each: 32x8192x8192 took 13.3 us so.) Slots in LDS are those of
-// the largest tile, and what is read behind the last row and block is as there; lane (r, g) takes chunks 2 g and 2 g + 1 of row r,
-// whose scales are one 16-bit word, the instruction's byte select taking them apart.
+// neighbouring lanes read different rows, 16 bytes of each: 32x8192x8192 took 13.3 us so.) With four waves the compiler
+// gives registers of the scales to addresses, and waits for all loads on their way before it asks for a wave's next unit:
+// the second buffer hides little there. Slots in LDS are those of the largest tile, and what is read behind the last row
+// and block is as there; lane (r, g) takes chunks 2 g and 2 g + 1 of row r, whose scales are one 16-bit word, the
+// instruction's byte select taking them apart.
 constexpr int rows_lds(int NP, int NQ, int WAVES) { return WAVES * 2 * (NP + NQ) * 16 * 128; }
 
 template <typename OutT, int NP, int NQ, int WAVES>
@@ -1069,7 +1071,8 @@ static int sliced(size_t items, F launch) {
 // run into the power limit (2048x1024: 10.6 against 12.4 us; 2048x2048: 17.5 and 12.7; 4096x2560: 48, 38 and 34;
 // 4096x4096: 74, 51 and 42). The proportions hold for other K but for short ones, where all store more than they
 // multiply and 128 and 256 are within a fifth of each other (4096x4096x1024: 21.7 and 23.3 us to fp32;
-// 8192x8192x512: 61 and 65, to bf16 53 and 43).
+// 8192x8192x512: 61 and 65, to bf16 53 and 43). Here and below the CUs are those of the whole card; on a partition of it,
+// which has fewer, the same kernels run and none of this was measured.
 static int tile_size(int64_t M, int64_t N, int64_t nb) {
   const int64_t least = M < N ? M : N;
   if (least < 64 || nb > 1 << 20) return 0;   // whole tiles inside C, 32-bit offsets in a tile

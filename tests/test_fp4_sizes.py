@@ -112,6 +112,31 @@ def test_product_over_an_empty_k_behind_32_bits(gpu, fp32, dtype):
     assert nonzero(out) == 0
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,nb", [(1 << 27, 1, 1), (3, 1 << 27, 1), (1, 2, 1 << 27)])
+def test_products_of_the_documented_sizes(gpu, M, N, nb):
+    """The largest of each size; exact, since what is not zero is little."""
+    def sparse(rows, seed):
+        q = torch.zeros(rows, 16 * nb, device=gpu, dtype=torch.uint8)
+        s = torch.full((rows, nb), 127, device=gpu, dtype=torch.uint8)
+        at = sorted({0, 1, rows // 2, rows - 2, rows - 1} & set(range(rows)))
+        blocks = sorted({0, 7, nb // 3, nb // 2, nb - 9, nb - 1} & set(range(nb)))
+        dense = torch.zeros(len(at), 32 * len(blocks), dtype=torch.float64)
+        for i, b in enumerate(blocks):
+            pick, scale = operand(len(at), 1, seed + i)
+            q[at, b * 16:b * 16 + 16], s[at, b:b + 1] = pick, scale
+            dense[:, 32 * i:32 * i + 32] = values_of(pick, scale)
+        return q, s, at, dense
+
+    a, sa, at_a, va = sparse(M, 1)
+    b, sb, at_b, vb = sparse(N, 50)
+    want = (va @ vb.t()).float()
+    for fp32, dtype in ((True, torch.float32), (False, torch.bfloat16)):
+        out = hk.gemm_mxfp4_nt(a, sa, b, sb, out_fp32=fp32)
+        assert torch.equal(out[at_a][:, at_b].cpu(), want.to(dtype))
+        assert nonzero(out) == want.count_nonzero().item()
+
+
 def test_rows_that_no_memory_holds_are_refused():
     try:
         L = hk.load()
